@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define OTTER_HIP_ABI_VERSION 14
+#define OTTER_HIP_ABI_VERSION 15
 
 /* element type codes */
 #define OTTER_DT_BF16 0
@@ -327,6 +327,52 @@ int otter_resize_bicubic_u8(const unsigned char* src, int n, int src_h, int src_
 int otter_action_step(const float* delta_chunks, const double* cur_pose, double* abs_chunks, double* ring, int* counts,
                       double* action10, double* robot7, int n_episodes, int horizon, int action_dim, int exec_horizon,
                       int receding, double k, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * K/V cache held in 4 or 8 bits: written, read back, attended to.  A quantised form of the GPU-resident history of
+ * transformer.py:76-104 / otter.py:153-175 (the reference keeps fp32 inputs and recomputes); no window limit.
+ *
+ * A row of the cache (one position, one key head) is head_dim numbers (32, 64, 96 or 128) in blocks of 32, each block 32 codes
+ * times a power of two: codes are e2m1 (4 bits, two a byte, even dimension in the low half) or e4m3 (8 bits); the scale byte is
+ * e + 127 with e the smallest integer in [-100, 100] at which the block's largest magnitude is at most 6 * 2^e (448 * 2^e); a
+ * code is the nearest one, ties to even.  A block with a NaN or an infinity gets scale byte 255 and reads back as NaN.
+ * --------------------------------------------------------------------------------------------------------------- */
+typedef struct otter_kv_cache {
+    unsigned char* codes;  long code_kv, code_episode, code_head;     /* byte strides: keys -> values, episode, head; a head's rows (head_dim * bits / 8 bytes each) are contiguous */
+    unsigned char* scales; long scale_kv, scale_episode, scale_head;  /* 4 bytes a row, byte b = scale of block b; contiguous over a head's rows */
+    int bits;                                                         /* 4 or 8 */
+    int episodes, heads, capacity, head_dim;                          /* capacity: positions per episode */
+} otter_kv_cache;
+/* Which cache rows a call is about: step t < count[i] of row i is window position pos[e] + t of episode e = idx[i].
+ * idx NULL: e = i; pos NULL: 0; count NULL: steps.  All device int32.  A row whose episode is outside [0, episodes), and a
+ * position outside [0, capacity), does not exist: it is not written, reads as zeros and is attended to by nobody. */
+typedef struct otter_kv_rows {
+    const int* idx;    /* [n_rows] */
+    const int* pos;    /* [episodes] */
+    const int* count;  /* [n_rows] */
+    int n_rows, steps;
+} otter_kv_rows;
+/* element (i, t, h, d) = p[i*row + t*step + h*head + d], strides in elements; OTTER_DT_* given by the call */
+typedef struct otter_kv_operand { void* p; long row, step, head; } otter_kv_operand;
+
+/* k and v (read only) into the cache.  An episode listed more than once: only its last listing is written. */
+int otter_kv_cache_write(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* k,
+                         const otter_kv_operand* v, void* stream);
+/* the cache's numbers into k and v; rows that do not exist become zeros.  fp16: cut at +-65504. */
+int otter_kv_cache_read(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* k,
+                        const otter_kv_operand* v, void* stream);
+/* softmax(scale q k^T) v over the cached positions.  Query t of row i is at position x = pos[e] + t and sees the positions
+ * 0 .. x (causal) or 0 .. pos[e] + count[i] - 1 (not causal), of these only the last `window` up to that position (0: all) and
+ * only those below max_len (what the caller knows about its lengths; capacity if nothing) and capacity.  A query that sees
+ * nothing, and every t >= count[i], gives zeros.  q, out: q_heads heads, a multiple of the cache's; query head j reads key head
+ * j / (q_heads / heads).
+ * k_new / v_new (both or none; steps == 1, count NULL): the step's own key and value, quantised, stored at pos[e] and attended to by the
+ * same launch -- as otter_kv_cache_write followed by this call.
+ * workspace: otter_attn_cache_workspace_floats(...) floats, 8-byte aligned, private to the call until it has run (0: none). */
+long otter_attn_cache_workspace_floats(int n_rows, int steps, int q_heads, int kv_heads, int head_dim, int window, int max_len);
+int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* q, int q_heads,
+                     const otter_kv_operand* k_new, const otter_kv_operand* v_new, const otter_kv_operand* out, int causal,
+                     int window, int max_len, float scale, float* workspace, long workspace_floats, void* stream);
 
 #ifdef __cplusplus
 }

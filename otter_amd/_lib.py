@@ -11,7 +11,7 @@ from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_lon
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("OTTER_HIP_LIB") or os.path.join(_HERE, "libotter_hip.so")
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 DT_BF16, DT_F16, DT_F32 = 0, 1, 2
 
@@ -39,7 +39,25 @@ class ReadoutProblem(Structure):
                 ("n_obs", c_int), ("nk", c_int), ("readouts", c_int), ("d", c_int), ("heads", c_int), ("hidden", c_int)]
 
 
+class KvCache(Structure):
+    """``otter_kv_cache``: the buffers of one quantised K/V cache."""
+    _fields_ = [("codes", c_void_p), ("code_kv", c_long), ("code_episode", c_long), ("code_head", c_long),
+                ("scales", c_void_p), ("scale_kv", c_long), ("scale_episode", c_long), ("scale_head", c_long),
+                ("bits", c_int), ("episodes", c_int), ("heads", c_int), ("capacity", c_int), ("head_dim", c_int)]
+
+
+class KvRows(Structure):
+    """``otter_kv_rows``: which cache rows a call is about."""
+    _fields_ = [("idx", c_void_p), ("pos", c_void_p), ("count", c_void_p), ("n_rows", c_int), ("steps", c_int)]
+
+
+class KvOperand(Structure):
+    """``otter_kv_operand``: a (row, step, head, dim) tensor with element strides."""
+    _fields_ = [("p", c_void_p), ("row", c_long), ("step", c_long), ("head", c_long)]
+
+
 _P, _I, _L, _F = c_void_p, c_int, c_long, c_float
+_KC, _KR, _KO = POINTER(KvCache), POINTER(KvRows), POINTER(KvOperand)
 
 _SIGNATURES = {
     "otter_gemm": [_I, _P, _L, _P, _I, _P, _P, _L, _P, _L, _I, _I, _I, _I, _P],
@@ -69,6 +87,10 @@ _SIGNATURES = {
     "otter_window_append": [_P, _P, _P, _P, _P, _I, _I, _I, _P],
     "otter_resize_bicubic_u8": [_P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _P, _P, _I, _P, _P, _I, _P],
     "otter_action_step": [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, c_double, _P],
+    # quantised K/V cache
+    "otter_kv_cache_write": [_KC, _KR, _I, _KO, _KO, _P],
+    "otter_kv_cache_read": [_KC, _KR, _I, _KO, _KO, _P],
+    "otter_attn_cache": [_KC, _KR, _I, _KO, _I, _KO, _KO, _KO, _I, _I, _I, _F, _P, _L, _P],
     # training step
     "otter_sgemm_strided": [_P, _L, _L, _P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _P, _P],
     "otter_act_fwd": [_P, _P, _L, _I, _P],
@@ -118,6 +140,8 @@ def load() -> ctypes.CDLL:
     lib.otter_gemm_static_ws_max_n.argtypes = []
     lib.otter_gemm_static_ws_init.restype = c_int
     lib.otter_gemm_static_ws_init.argtypes = []
+    lib.otter_attn_cache_workspace_floats.restype = c_long
+    lib.otter_attn_cache_workspace_floats.argtypes = [c_int] * 7
     _lib = lib
     return lib
 
@@ -132,4 +156,4 @@ def call(name: str, *args) -> None:
 def exported_names():
     return sorted(list(_SIGNATURES) + ["otter_last_error", "otter_hip_abi_version", "otter_grad_stats_workspace_floats",
                                             "otter_pos_emb_packed_elems", "otter_gemm_workspace_floats", "otter_gemm_static_ws_max_n",
-                                            "otter_gemm_static_ws_init"])
+                                            "otter_gemm_static_ws_init", "otter_attn_cache_workspace_floats"])

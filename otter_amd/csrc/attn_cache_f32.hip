@@ -1,0 +1,6 @@
+// attn_cache.hpp for float activations.
+#include <type_traits>
+#define OTTER_ATTN_CACHE_IMPL
+#include "attn_cache.hpp"
+
+template int otter_attn_cache_launch<float>(const AttnCacheArgs&, int, int, int, unsigned, hipStream_t);

@@ -1,0 +1,196 @@
+// Writing the quantised K/V cache and reading it back (layout and arithmetic: kv_cache.hpp).
+#include "kv_cache.hpp"
+
+namespace {
+
+// Both kernels move 8 numbers a lane: a lane's codes are 4 (or 8) bytes, four lanes share a block and its scale.  Lanes run
+// along the head dimension, then along the steps, then along the heads: a cache row is contiguous with the row of the next
+// step, so a wave's codes form one run of 256 (512) bytes or more, and its numbers runs of head_dim elements.
+// Memory-bound: head_dim * (element size + BITS / 8) + 4 bytes a row, no reuse.
+template <int NB, int BITS, typename T>
+__global__ __launch_bounds__(256) void kv_write_kernel(KvGeom g, KvOperand<const T> k, KvOperand<const T> v, int vec) {
+    constexpr int P = 4 * NB, RB = 4 * NB * BITS;                   // lanes and bytes per row
+    const int id = blockIdx.x * 256 + threadIdx.x;
+    const int unit = id / P, p = id % P;                            // P divides a quad evenly: a block's four lanes are neighbours
+    const int h = unit / g.T, t = unit - h * g.T;
+    const int kv = blockIdx.y;
+    for (int i = blockIdx.z; i < g.n; i += gridDim.z) {
+        const KvRow r = kv_row(g, i);
+        const int at = r.pos + t;
+        bool live = h < g.H && r.e >= 0 && t < r.cnt && at >= 0 && at < g.S;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (live) {
+            const KvOperand<const T>& o = kv ? v : k;
+            kv_load8<T>(o.p + (long)i * o.row + (long)t * o.step + (long)h * o.head + 8 * p, vec, x);
+        }
+        if (g.idx && r.e >= 0 && i + 1 < g.n) {                                    // an episode listed twice: the last listing is the one that is written
+            bool later = false;
+            for (int j = i + 1 + (int)threadIdx.x; j < g.n; j += 256) later |= g.idx[j] == r.e;
+            if (__syncthreads_or(later)) continue;
+        }
+        const unsigned sb = kv_scale_byte<BITS>(kv_block_top(x));
+        unsigned w[BITS / 4];
+        kv_encode8<BITS>(x, sb, w);
+        if (live) {
+            unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h * g.ch + (long)at * RB + p * BITS;
+            if constexpr (BITS == 4) *(unsigned*)c = w[0];
+            else *(uint2*)c = make_uint2(w[0], w[1]);
+            if ((p & 3) == 0) g.scales[kv * g.skv + (long)r.e * g.se + (long)h * g.sh + (long)at * 4 + (p >> 2)] = (unsigned char)sb;
+        }
+    }
+}
+
+template <int BITS> __device__ __forceinline__ void kv_decode8(const unsigned (&w)[BITS / 4], unsigned scale_byte, float (&x)[8]) {
+    const float sc = __uint_as_float(scale_byte << 23);
+    f32x2 y[4];
+    if constexpr (BITS == 4) {
+        y[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 0);
+        y[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 1);
+        y[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 2);
+        y[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 3);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            y[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[h], sc, false);
+            y[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[h], sc, true);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i >> 1][i & 1];
+}
+
+template <typename T> __device__ __forceinline__ void kv_store8(T* p, bool vec, const float (&x)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        if (vec) {
+            *(f32x4*)p = (f32x4){x[0], x[1], x[2], x[3]};
+            *(f32x4*)(p + 4) = (f32x4){x[4], x[5], x[6], x[7]};
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = x[i];
+    } else {
+        typename Half16<T>::v8 o;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)                                // exact in bf16; fp16: rounded below 2^-14, cut at its largest number (NaN stays)
+            o[i] = (T)(sizeof(T) == 2 && KvElem<T>::code == DT_F16 && x[i] == x[i] ? __builtin_amdgcn_fmed3f(x[i], -65504.f, 65504.f) : x[i]);
+        if (vec) { *(typename Half16<T>::v8*)p = o; return; }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = o[i];
+    }
+}
+
+template <int NB, int BITS, typename T>
+__global__ __launch_bounds__(256) void kv_read_kernel(KvGeom g, KvOperand<T> k, KvOperand<T> v, int vec) {
+    constexpr int P = 4 * NB, RB = 4 * NB * BITS;
+    const int id = blockIdx.x * 256 + threadIdx.x;
+    const int unit = id / P, p = id % P;
+    const int h = unit / g.T, t = unit - h * g.T;
+    if (h >= g.H) return;
+    const int kv = blockIdx.y;
+    for (int i = blockIdx.z; i < g.n; i += gridDim.z) {
+        const KvRow r = kv_row(g, i);
+        const int at = r.pos + t;
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (r.e >= 0 && t < r.cnt && at >= 0 && at < g.S) {
+            const unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h * g.ch + (long)at * RB + p * BITS;
+            const unsigned sb = g.scales[kv * g.skv + (long)r.e * g.se + (long)h * g.sh + (long)at * 4 + (p >> 2)];
+            unsigned w[BITS / 4];
+            if constexpr (BITS == 4) w[0] = *(const unsigned*)c;
+            else { const uint2 u = *(const uint2*)c; w[0] = u.x; w[1] = u.y; }
+            kv_decode8<BITS>(w, sb, x);
+        }
+        const KvOperand<T>& o = kv ? v : k;
+        kv_store8<T>(o.p + (long)i * o.row + (long)t * o.step + (long)h * o.head + 8 * p, vec, x);
+    }
+}
+
+inline bool operand_vec(const otter_kv_operand* o, int dtype) {
+    const long es = dtype == DT_F32 ? 4 : 2;
+    return aligned16(o->p) && (o->row * es) % 16 == 0 && (o->step * es) % 16 == 0 && (o->head * es) % 16 == 0;
+}
+
+template <bool WRITE, int NB, int BITS, typename T>
+void launch(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
+    const long lanes = (long)g.H * g.T * 4 * NB;
+    const dim3 grid((unsigned)((lanes + 255) / 256), 2, (unsigned)min(g.n, 65535));
+    if constexpr (WRITE)
+        hipLaunchKernelGGL((kv_write_kernel<NB, BITS, T>), grid, dim3(256), 0, s, g, (KvOperand<const T>{(const T*)k->p, k->row, k->step, k->head}),
+                           (KvOperand<const T>{(const T*)v->p, v->row, v->step, v->head}), vec);
+    else
+        hipLaunchKernelGGL((kv_read_kernel<NB, BITS, T>), grid, dim3(256), 0, s, g, (KvOperand<T>{(T*)k->p, k->row, k->step, k->head}),
+                           (KvOperand<T>{(T*)v->p, v->row, v->step, v->head}), vec);
+}
+
+template <bool WRITE, int BITS, typename T>
+void launch_nb(int nb, const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
+    if (nb == 1) launch<WRITE, 1, BITS, T>(g, k, v, vec, s);
+    else if (nb == 2) launch<WRITE, 2, BITS, T>(g, k, v, vec, s);
+    else if (nb == 3) launch<WRITE, 3, BITS, T>(g, k, v, vec, s);
+    else launch<WRITE, 4, BITS, T>(g, k, v, vec, s);
+}
+
+template <bool WRITE>
+int move(const otter_kv_cache* c, const otter_kv_rows* r, int dtype, const otter_kv_operand* k, const otter_kv_operand* v, hipStream_t s, const char* name) {
+    if (int rc = otter_kv_check(c, r, name)) return rc;
+    if (r->n_rows == 0 || r->steps == 0) return OTTER_OK;
+    if (int rc = otter_kv_check_operand(k, dtype, !WRITE, "k", name)) return rc;
+    if (int rc = otter_kv_check_operand(v, dtype, !WRITE, "v", name)) return rc;
+    OTTER_REQUIRE((long)c->heads * r->steps * (c->head_dim / 8) < (1L << 31) - 256, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: %d heads x %d steps too large", name, c->heads, r->steps);
+    const KvGeom g = otter_kv_geom(c, r);
+    const int vec = operand_vec(k, dtype) && operand_vec(v, dtype), nb = c->head_dim / 32;
+    if (c->bits == 4) {
+        if (dtype == DT_F32) launch_nb<WRITE, 4, float>(nb, g, k, v, vec, s);
+        else if (dtype == DT_BF16) launch_nb<WRITE, 4, __bf16>(nb, g, k, v, vec, s);
+        else launch_nb<WRITE, 4, _Float16>(nb, g, k, v, vec, s);
+    } else {
+        if (dtype == DT_F32) launch_nb<WRITE, 8, float>(nb, g, k, v, vec, s);
+        else if (dtype == DT_BF16) launch_nb<WRITE, 8, __bf16>(nb, g, k, v, vec, s);
+        else launch_nb<WRITE, 8, _Float16>(nb, g, k, v, vec, s);
+    }
+    OTTER_CHECK_LAUNCH(name);
+    return OTTER_OK;
+}
+
+}  // namespace
+
+int otter_kv_check(const otter_kv_cache* c, const otter_kv_rows* r, const char* name) {
+    OTTER_REQUIRE(c && r && c->codes && c->scales, OTTER_ERR_INVALID_ARGUMENT, "%s: null cache", name);
+    OTTER_REQUIRE(c->bits == 4 || c->bits == 8, OTTER_ERR_INVALID_ARGUMENT, "%s: %d bits (4 or 8)", name, c->bits);
+    OTTER_REQUIRE(c->head_dim >= 32 && c->head_dim <= 128 && c->head_dim % 32 == 0, OTTER_ERR_UNSUPPORTED_SHAPE,
+                  "%s: head_dim=%d must be 32, 64, 96 or 128", name, c->head_dim);
+    OTTER_REQUIRE(c->episodes >= 0 && c->heads > 0 && c->capacity > 0 && c->capacity <= (1 << 30), OTTER_ERR_INVALID_ARGUMENT,
+                  "%s: episodes=%d heads=%d capacity=%d", name, c->episodes, c->heads, c->capacity);
+    const long row = (long)c->head_dim * c->bits / 8;
+    OTTER_REQUIRE(aligned16(c->codes) && c->code_kv % 16 == 0 && c->code_episode % 16 == 0 && c->code_head % 16 == 0, OTTER_ERR_ALIGNMENT,
+                  "%s: codes and their strides must be multiples of 16 bytes", name);
+    OTTER_REQUIRE((reinterpret_cast<uintptr_t>(c->scales) & 3u) == 0 && c->scale_kv % 4 == 0 && c->scale_episode % 4 == 0 && c->scale_head % 4 == 0,
+                  OTTER_ERR_ALIGNMENT, "%s: scales and their strides must be multiples of 4 bytes", name);
+    OTTER_REQUIRE((c->heads == 1 || c->code_head >= c->capacity * row) && (c->heads == 1 || c->scale_head >= c->capacity * 4L),
+                  OTTER_ERR_INVALID_ARGUMENT, "%s: heads of the cache overlap", name);
+    OTTER_REQUIRE(r->n_rows >= 0 && r->steps >= 0 && r->steps <= (1 << 30), OTTER_ERR_INVALID_ARGUMENT, "%s: n_rows=%d steps=%d", name, r->n_rows, r->steps);
+    OTTER_REQUIRE(r->idx || r->n_rows <= c->episodes, OTTER_ERR_INVALID_ARGUMENT, "%s: %d rows without idx, cache of %d episodes", name, r->n_rows, c->episodes);
+    return OTTER_OK;
+}
+
+int otter_kv_check_operand(const otter_kv_operand* o, int dtype, bool write, const char* what, const char* name) {
+    OTTER_REQUIRE(dtype == DT_BF16 || dtype == DT_F16 || dtype == DT_F32, OTTER_ERR_INVALID_ARGUMENT, "%s: unknown dtype %d", name, dtype);
+    OTTER_REQUIRE(o && o->p, OTTER_ERR_INVALID_ARGUMENT, "%s: null operand %s", name, what);
+    OTTER_REQUIRE((reinterpret_cast<uintptr_t>(o->p) & (dtype == DT_F32 ? 3u : 1u)) == 0, OTTER_ERR_ALIGNMENT, "%s: %s is not aligned to its elements", name, what);
+    OTTER_REQUIRE(!write || (o->row >= 0 && o->step >= 0 && o->head >= 0), OTTER_ERR_INVALID_ARGUMENT, "%s: negative strides of %s", name, what);
+    return OTTER_OK;
+}
+
+KvGeom otter_kv_geom(const otter_kv_cache* c, const otter_kv_rows* r) {
+    return KvGeom{c->codes, c->code_kv, c->code_episode, c->code_head, c->scales, c->scale_kv, c->scale_episode, c->scale_head,
+                  c->episodes, c->capacity, c->heads, r->idx, r->pos, r->count, r->n_rows, r->steps};
+}
+
+extern "C" int otter_kv_cache_write(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* k,
+                                    const otter_kv_operand* v, void* stream) {
+    return move<true>(cache, rows, dtype, k, v, (hipStream_t)stream, "otter_kv_cache_write");
+}
+
+extern "C" int otter_kv_cache_read(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* k,
+                                   const otter_kv_operand* v, void* stream) {
+    return move<false>(cache, rows, dtype, k, v, (hipStream_t)stream, "otter_kv_cache_read");
+}

@@ -622,6 +622,161 @@ def action_step(delta_chunks: Tensor, cur_pose: Tensor, ring: Tensor, counts: Te
     return robot, act10, abs_chunks
 
 
+# ------------------------------------------------------------------------------------------------------ quantised K/V cache
+def _kv_operand(t: Tensor, dtype, shape: tuple, name: str, device) -> "_lib.KvOperand":
+    """A (row, step, head, dim) tensor with free strides outside the last dimension."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or tuple(t.shape) != shape:
+        _chk(t, dtype, name)
+        raise ValueError(f"{name}: {tuple(t.shape)} on {t.device}, expected {shape} on {device}")
+    sr, ss, sh, sd = t.stride()
+    if sd != 1:
+        raise ValueError(f"{name}: innermost dimension must be contiguous")
+    n, steps, h, _ = shape
+    return _lib.KvOperand(t.data_ptr(), sr if n > 1 else 0, ss if steps > 1 else 0, sh if h > 1 else 0)
+
+
+def _kv_cache(codes: Tensor, scales: Tensor, head_dim: int, name: str) -> "_lib.KvCache":
+    _chk(codes, torch.uint8, name + ".codes", 5)
+    _chk(scales, torch.uint8, name + ".scales", 5)
+    two, e, h, s, row = codes.shape
+    bits = {head_dim // 2: 4, head_dim: 8}.get(row)
+    if two != 2 or tuple(scales.shape) != (2, e, h, s, 4) or bits is None or scales.device != codes.device:
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} for head_dim {head_dim}: "
+                         "(2, episodes, heads, capacity, head_dim / 2 or head_dim) and (2, episodes, heads, capacity, 4)")
+    if head_dim % 32 != 0 or not 32 <= head_dim <= 128:
+        raise ValueError(f"{name}: head_dim {head_dim} must be 32, 64, 96 or 128")
+    if s == 0 or h == 0:
+        raise ValueError(f"{name}: the cache holds no positions or no heads")
+    cs, ss = codes.stride(), scales.stride()
+    if (s > 1 and (cs[3] != row or ss[3] != 4)) or cs[4] != 1 or ss[4] != 1:
+        raise ValueError(f"{name}: the positions of a head must be contiguous")
+    return _lib.KvCache(codes.data_ptr(), cs[0], cs[1] if e > 1 else 0, cs[2] if h > 1 else 0,
+                        scales.data_ptr(), ss[0], ss[1] if e > 1 else 0, ss[2] if h > 1 else 0, bits, e, h, s, head_dim)
+
+
+def _kv_index(t: Optional[Tensor], length: int, name: str, device) -> Optional[int]:
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != length or not t.is_contiguous():
+        _chk(t, torch.int32, name, 1)
+        raise ValueError(f"{name}: {tuple(t.shape)} on {t.device}, expected a contiguous ({length},) on {device}")
+    return t.data_ptr()
+
+
+def _kv_rows(cache: "_lib.KvCache", device, n: int, steps: int, pos: Optional[Tensor], idx: Optional[Tensor], count: Optional[Tensor],
+             name: str) -> "_lib.KvRows":
+    if idx is None and n > cache.episodes:
+        raise ValueError(f"{name}: {n} rows without idx, cache of {cache.episodes} episodes")
+    return _lib.KvRows(_kv_index(idx, n, name + ".idx", device), _kv_index(pos, cache.episodes, name + ".pos", device),
+                       _kv_index(count, n, name + ".count", device), n, steps)
+
+
+def _kv_call(device, fn: str, *args) -> None:
+    """Launch on the cache's device, on that device's current stream."""
+    if device.index == torch.cuda.current_device():
+        _lib.call(fn, *args, _stream())
+    else:
+        with torch.cuda.device(device):
+            _lib.call(fn, *args, _stream())
+
+
+def kv_cache_write(k: Tensor, v: Tensor, codes: Tensor, scales: Tensor, pos: Optional[Tensor] = None, idx: Optional[Tensor] = None,
+                   count: Optional[Tensor] = None) -> None:
+    """Quantise keys and values (n, steps, heads, head_dim) -- fp32 / bf16 / fp16, any strides outside the last dimension -- into
+    a cache: ``codes`` uint8 (2, episodes, heads, capacity, head_dim / 2 for 4 bits or head_dim for 8), ``scales`` uint8
+    (2, episodes, heads, capacity, 4); see ``otter_kv_cache`` for the format.  Step t < count[i] of row i goes to position
+    pos[e] + t of episode e = idx[i].  ``pos`` int32 (episodes,), ``idx`` and ``count`` int32 (n,); None: zeros, row i = episode i,
+    all steps.  What lies outside the cache is not written; an episode listed twice gets its last listing."""
+    if not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError("kv_cache_write: k must be (n, steps, heads, head_dim)")
+    n, steps, h, d = k.shape
+    dt = _dt(k.dtype, "kv_cache_write.k")
+    c = _kv_cache(codes, scales, d, "kv_cache_write")
+    dev = codes.device
+    if h != c.heads:
+        raise ValueError(f"kv_cache_write: {h} heads, cache of {c.heads}")
+    ko, vo = _kv_operand(k, k.dtype, (n, steps, h, d), "kv_cache_write.k", dev), _kv_operand(v, k.dtype, (n, steps, h, d), "kv_cache_write.v", dev)
+    r = _kv_rows(c, dev, n, steps, pos, idx, count, "kv_cache_write")
+    if n and steps:
+        _kv_call(dev, "otter_kv_cache_write", c, r, dt, ko, vo)
+
+
+def kv_cache_read(codes: Tensor, scales: Tensor, head_dim: int, steps: int, pos: Optional[Tensor] = None, idx: Optional[Tensor] = None,
+                  count: Optional[Tensor] = None, *, n_rows: Optional[int] = None, dtype=torch.float32):
+    """The numbers that positions pos[e] .. pos[e] + steps - 1 of the listed episodes hold: (k, v), each (n, steps, heads, head_dim)
+    in ``dtype``; rows as in :func:`kv_cache_write` (without ``idx``: the first ``n_rows`` episodes, all by default).  What the
+    cache does not hold, and steps at or past count[i], read as zeros."""
+    dt = _dt(dtype, "kv_cache_read.dtype")
+    c = _kv_cache(codes, scales, head_dim, "kv_cache_read")
+    dev = codes.device
+    if steps < 0:
+        raise ValueError("kv_cache_read: negative steps")
+    n = idx.shape[0] if idx is not None else c.episodes if n_rows is None else int(n_rows)
+    r = _kv_rows(c, dev, n, int(steps), pos, idx, count, "kv_cache_read")
+    k = torch.empty(n, steps, c.heads, head_dim, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    if n and steps:
+        sr, ss, sh, _ = k.stride()
+        _kv_call(dev, "otter_kv_cache_read", c, r, dt, _lib.KvOperand(k.data_ptr(), sr, ss, sh), _lib.KvOperand(v.data_ptr(), sr, ss, sh))
+    return k, v
+
+
+def _attn_cache(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], codes, scales, pos, idx, count, causal: bool, window: int,
+                scale: Optional[float], max_len: Optional[int], name: str) -> Tensor:
+    n, steps, hq, d = q.shape
+    dt = _dt(q.dtype, name + ".q")
+    c = _kv_cache(codes, scales, d, name)
+    dev = codes.device
+    if hq == 0 or hq % c.heads != 0:
+        raise ValueError(f"{name}: {hq} query heads over {c.heads} key heads")
+    if window < 0 or (max_len is not None and max_len < 1):
+        raise ValueError(f"{name}: window={window}, max_len={max_len}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 3.0e38:
+        raise ValueError(f"{name}: scale must be positive and finite")
+    cap = c.capacity if max_len is None else min(int(max_len), c.capacity)
+    qo = _kv_operand(q, q.dtype, (n, steps, hq, d), name + ".q", dev)
+    ko = vo = None
+    if k is not None:
+        ko, vo = _kv_operand(k, q.dtype, (n, 1, c.heads, d), name + ".k", dev), _kv_operand(v, q.dtype, (n, 1, c.heads, d), name + ".v", dev)
+    r = _kv_rows(c, dev, n, steps, pos, idx, count, name)
+    out = torch.empty(n, steps, hq, d, dtype=q.dtype, device=dev)
+    if n == 0 or steps == 0:
+        return out
+    if c.episodes == 0:
+        raise ValueError(f"{name}: the cache has no episodes")
+    need = _lib.load().otter_attn_cache_workspace_floats(n, steps, hq, c.heads, d, window, cap)
+    # the call's own scratch, from the allocator of the stream (or the graph being captured) it runs on
+    ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
+    _kv_call(dev, "otter_attn_cache", c, r, dt, qo, hq, ko, vo, _lib.KvOperand(out.data_ptr(), steps * hq * d, hq * d, d), int(bool(causal)),
+             window, cap, scale, None if ws is None else ws.data_ptr(), need)
+    return out
+
+
+def attn_cache(q: Tensor, codes: Tensor, scales: Tensor, pos: Optional[Tensor] = None, idx: Optional[Tensor] = None,
+               count: Optional[Tensor] = None, *, causal: bool = True, window: int = 0, scale: Optional[float] = None,
+               max_len: Optional[int] = None) -> Tensor:
+    """Attention over a quantised cache (see :func:`kv_cache_write`): q (n, steps, q_heads, head_dim) fp32 / bf16 / fp16 -> the same
+    shape and type.  Query t of row i sits at position x = pos[e] + t of episode e = idx[i] and sees positions 0 .. x (``causal``)
+    or 0 .. pos[e] + count[i] - 1, of these the last ``window`` (0: all), and none at or past ``max_len`` (an upper bound that the
+    caller knows for its lengths: it sizes the launch; default: the capacity).  A query that sees nothing gives zeros, and so
+    do the steps at or past count[i].  Query head j reads key head j // (q_heads // heads); ``scale`` defaults to head_dim ** -0.5."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("attn_cache: q must be (n, steps, q_heads, head_dim)")
+    return _attn_cache(q, None, None, codes, scales, pos, idx, count, causal, int(window), scale, max_len, "attn_cache")
+
+
+def attn_cache_rows(q: Tensor, k: Tensor, v: Tensor, codes: Tensor, scales: Tensor, pos: Optional[Tensor] = None,
+                    idx: Optional[Tensor] = None, *, window: int = 0, scale: Optional[float] = None, max_len: Optional[int] = None) -> Tensor:
+    """One new position per listed episode: k, v (n, heads, head_dim) are quantised into position pos[e] and q (n, q_heads, head_dim)
+    attends to the history with them, in one call -- :func:`kv_cache_write` followed by :func:`attn_cache`."""
+    for t, nm in ((q, "q"), (k, "k"), (v, "v")):
+        if not isinstance(t, torch.Tensor) or t.dim() != 3:
+            raise ValueError(f"attn_cache_rows: {nm} must be (n, heads, head_dim)")
+    return _attn_cache(q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), codes, scales, pos, idx, None, True, int(window), scale, max_len,
+                       "attn_cache_rows").squeeze(1)
+
+
 # ------------------------------------------------------------------------------------------------------ training step
 def _f32_2d(t: Tensor, name: str):
     _chk(t, torch.float32, name, 2)
