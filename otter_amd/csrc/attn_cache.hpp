@@ -13,9 +13,10 @@
 // (lane = key, head_dim / 4 consecutive numbers), V as 8 rows x head_dim / 16 numbers a lane and turned by v_perm after the
 // conversion.  Rows past the last key are never read (addresses are cut at it).
 //
-// Masked keys.  Scores are selected, but 0 * NaN of a masked value row would still reach the accumulator.  The fast pass ignores
-// that; if a wave ends with a non-finite accumulator it runs again with the value rows cleaned and NaN set where a row that the
-// column really sees is not finite.
+// Masked keys.  Scores are selected, but 0 * NaN of a masked value row would still reach the accumulator.  Only tiles at the end of
+// somebody's range have masked keys; where such a tile holds a scale byte that may stand for a non-finite block (>= 224; the
+// writer's finite ones end at 227) its value rows are cleaned before the product, and the column is marked if it really sees
+// one of them.  A lane's accumulators lie in one block of 32, so one mark a column is enough.
 #pragma once
 #include "kv_cache.hpp"
 
@@ -59,7 +60,6 @@ template <typename T> int otter_attn_cache_launch(const AttnCacheArgs& a, int nb
 namespace {
 
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
-typedef __attribute__((ext_vector_type(4), aligned(4))) unsigned u32x4_a4;     // 16 bytes at a 4-byte boundary
 
 // what one tile of 32 keys needs from memory, as loaded
 template <int NB, int BITS> struct RawTile {
@@ -70,63 +70,69 @@ template <int NB, int BITS> struct RawTile {
     unsigned ks[2], vs[8];                                         // scale words of the rows
 };
 
-template <int NB, int BITS> struct TileSource {
-    const unsigned char* kc; const unsigned char* vc;              // rows of this episode and head
-    const unsigned char* ksc; const unsigned char* vsc;
-};
+struct TileSource { const unsigned char* k; const unsigned char* v; const unsigned char* ks; const unsigned char* vs; };   // rows and scale words of this episode and head
 
 __device__ __forceinline__ int v_row(int g, int i) { return 4 * g + (i & 3) + 16 * (i >> 2); }   // key of element i of lane group g's operand
 
-template <int W> __device__ __forceinline__ void load_words(const unsigned char* p, unsigned (&w)[W]) {
-    if constexpr (W == 1) w[0] = *(const unsigned*)p;
-    else if constexpr (W == 2) { const uint2 u = *(const uint2*)p; w[0] = u.x; w[1] = u.y; }
-    else if constexpr (W == 3) {
-        typedef __attribute__((ext_vector_type(3), aligned(4))) unsigned u3;
-        const u3 u = *(const u3*)p;
-        w[0] = u[0]; w[1] = u[1]; w[2] = u[2];
-    } else if constexpr (W == 6) {
+// Rows are read through buffer resources that end with the tile's last existing row: what lies behind reads as zeros (checked
+// word by word; scale byte 0 with codes 0 is the number 0), so a ragged tile needs no addresses of its own, and every load is a
+// 32-bit lane offset from a scalar base.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const unsigned char* base, int k0, int row_bytes, int rows) {
+    const unsigned long long at = (unsigned long long)base + (unsigned long long)k0 * row_bytes;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)at), hi = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(min(rows, 32) * row_bytes), 0x00027000);
+}
+template <int BYTES, int W> __device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, unsigned (&w)[W]) {
+    if constexpr (BYTES == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b8(r, off, 0, 0);
+    else if constexpr (BYTES == 2) w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+    else if constexpr (BYTES == 4) w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    else if constexpr (BYTES == 8 || BYTES == 24) {
 #pragma unroll
-        for (int i = 0; i < 3; ++i) { const uint2 u = *(const uint2*)(p + 8 * i); w[2 * i] = u.x; w[2 * i + 1] = u.y; }
+        for (int i = 0; i < W; i += 2) { const auto u = __builtin_amdgcn_raw_buffer_load_b64(r, off + 4 * i, 0, 0); w[i] = u[0]; w[i + 1] = u[1]; }
+    } else if constexpr (BYTES == 12) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b96(r, off, 0, 0);
+        w[0] = u[0]; w[1] = u[1]; w[2] = u[2];
     } else {
 #pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const u32x4 u = *(const u32x4*)(p + 16 * i);
-            w[4 * i] = u[0]; w[4 * i + 1] = u[1]; w[4 * i + 2] = u[2]; w[4 * i + 3] = u[3];
+        for (int i = 0; i < W; i += 4) {
+            const auto u = __builtin_amdgcn_raw_buffer_load_b128(r, off + 4 * i, 0, 0);
+            w[i] = u[0]; w[i + 1] = u[1]; w[i + 2] = u[2]; w[i + 3] = u[3];
         }
     }
 }
-template <int BYTES, int W> __device__ __forceinline__ void load_part(const unsigned char* p, unsigned (&w)[W]) {
-    if constexpr (BYTES == 1) w[0] = *p;
-    else if constexpr (BYTES == 2) w[0] = *(const unsigned short*)p;
-    else load_words<W>(p, w);
-}
 
-// rows k0 .. k0 + 31 of the cache; TAIL: only nk of them exist, the others repeat the last one
-template <int NB, int BITS, bool TAIL>
-__device__ __forceinline__ void load_tile(RawTile<NB, BITS>& r, const TileSource<NB, BITS>& src, int k0, int nk, int lane) {
-    constexpr int RB = 4 * NB * BITS, KB = RB / 4, DV = RawTile<NB, BITS>::DV, VB = DV * BITS / 8;
+// key (value) rows k0 .. k0 + 31 of the cache, of which the first `rows` exist
+template <int NB, int BITS> __device__ __forceinline__ void load_keys(RawTile<NB, BITS>& r, const TileSource& src, int k0, int rows, int lane) {
+    constexpr int RB = 4 * NB * BITS, KB = RB / 4;
     const int li = lane & 15, g = lane >> 4;
-    const unsigned char* kc = src.kc + (long)k0 * RB;
-    const unsigned char* vc = src.vc + (long)k0 * RB;
-    const unsigned char* ksc = src.ksc + (long)k0 * 4;
-    const unsigned char* vsc = src.vsc + (long)k0 * 4;
-    const int vl = NB == 3 ? min(li, 11) * VB : li * VB;           // NB = 3: lanes 12 .. 15 repeat lane 11 (their output rows are not stored)
+    const auto kc = rows_of(src.k, k0, RB, rows), ks = rows_of(src.ks, k0, 4, rows);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int row = TAIL ? min(li + 16 * h, nk - 1) : li + 16 * h;
-        load_words(kc + row * RB + g * KB, r.k[h]);
-        r.ks[h] = *(const unsigned*)(ksc + row * 4);
+        buffer_words<KB>(kc, li * RB + g * KB + 16 * h * RB, r.k[h]);
+        r.ks[h] = __builtin_amdgcn_raw_buffer_load_b32(ks, li * 4 + 64 * h, 0, 0);
     }
-    if constexpr (TAIL) {
+}
+template <int NB, int BITS> __device__ __forceinline__ void load_values(RawTile<NB, BITS>& r, const TileSource& src, int k0, int rows, int lane) {
+    constexpr int RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, VB = DV * BITS / 8;
+    const int li = lane & 15, g = lane >> 4;
+    const auto vc = rows_of(src.v, k0, RB, rows), vs = rows_of(src.vs, k0, 4, rows);
+    const int vl = (NB == 3 ? min(li, 11) : li) * VB + 4 * g * RB;  // NB = 3: lanes 12 .. 15 repeat lane 11 (their output rows are not stored)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) r.vs[i] = *(const unsigned*)(vsc + min(v_row(g, i), nk - 1) * 4);
-    } else {
-        const u32x4_a4 a = *(const u32x4_a4*)(vsc + 16 * g), b = *(const u32x4_a4*)(vsc + 64 + 16 * g);
+    for (int h = 0; h < 2; ++h) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b128(vs, 16 * g + 64 * h, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { r.vs[i] = a[i]; r.vs[4 + i] = b[i]; }
+        for (int i = 0; i < 4; ++i) r.vs[4 * h + i] = u[i];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load_part<VB>(vc + (TAIL ? min(v_row(g, i), nk - 1) : v_row(g, i)) * RB + vl, r.v[i]);
+    for (int i = 0; i < 8; ++i) buffer_words<VB>(vc, vl + ((i & 3) + 16 * (i >> 2)) * RB, r.v[i]);
+}
+template <int BYTES, int W> __device__ __forceinline__ void lds_words(const unsigned char* p, unsigned (&w)[W]) {
+    if constexpr (BYTES == 1) w[0] = *p;
+    else if constexpr (BYTES == 2) w[0] = *(const unsigned short*)p;
+    else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = *(const unsigned*)(p + 4 * i);
+    }
 }
 
 // scale operand of a block conversion: the wanted byte moved to the exponent's place (the conversion reads nothing else)
@@ -211,55 +217,32 @@ template <int NB, int BITS, typename T, int QT> struct WaveState {
     }
 };
 
-template <int NB, int BITS, typename T, int QT, bool CAREFUL>
-__device__ __forceinline__ void tile_step(const RawTile<NB, BITS>& r, WaveState<NB, BITS, T, QT>& st, const bf16x8 (&qf)[QT][AttnTerms<T>::q][NB],
-                                          int k0, bool masked, const int (&lo)[QT], const int (&hi)[QT], float c, int lane) {
-    constexpr int NQ = AttnTerms<T>::q, NP = AttnTerms<T>::p, DV = RawTile<NB, BITS>::DV;
-    const int li = lane & 15, g = lane >> 4;
-    f32x4 s[QT][2];
+// scores of 32 keys: element i of s[t] belongs to key v_row(g, i) and the lane's column t
+template <int NB, int BITS, typename T, int QT>
+__device__ __forceinline__ void tile_scores(const RawTile<NB, BITS>& r, const bf16x8 (&qf)[QT][AttnTerms<T>::q][NB], f32x4 (&s)[QT][2], int lane) {
+    constexpr int NQ = AttnTerms<T>::q;
+    const int g = lane >> 4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        bf16x8 kf[NB];
 #pragma unroll
-        for (int j = 0; j < NB; ++j)                               // unit NB g + j of 8 numbers lies in block (NB g + j) / 4
-            kf[j] = decode8<BITS>(&r.k[h][j * BITS / 4], scale_of(r.ks[h], NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2));
+        for (int t = 0; t < QT; ++t) s[t][h] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            s[t][h] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NB; ++j) {                             // unit NB g + j of 8 numbers lies in block (NB g + j) / 4
+            const bf16x8 kf = decode8<BITS>(&r.k[h][j * BITS / 4], scale_of(r.ks[h], NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2));
 #pragma unroll
-            for (int n = NQ - 1; n >= 0; --n)                      // small terms first
+            for (int t = 0; t < QT; ++t)
 #pragma unroll
-                for (int j = 0; j < NB; ++j) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[j], qf[t][n][j], s[t][h], 0, 0, 0);
+                for (int n = NQ - 1; n >= 0; --n) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][n][j], s[t][h], 0, 0, 0);
         }
     }
-    // value rows: 8 keys x DV numbers a lane -> DV operands of 8 keys
-    u32x4 vf[DV];
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        const int block = NB == 1 ? 0 : NB == 2 ? li >> 3 : li >> 2;
-        const float s0 = scale_of(r.vs[i], block), s1 = scale_of(r.vs[i + 1], block);
-#pragma unroll
-        for (int j = 0; j < DV / 2; ++j) {
-            const unsigned a = decode_pair<BITS>(r.v[i], j, s0), b = decode_pair<BITS>(r.v[i + 1], j, s1);
-            vf[2 * j][i >> 1] = __builtin_amdgcn_perm(b, a, 0x05040100u);
-            vf[2 * j + 1][i >> 1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-        }
-    }
-    bf16x8 bad[CAREFUL ? DV : 1];
-    if constexpr (CAREFUL) {
-#pragma unroll
-        for (int j = 0; j < DV; ++j) {
-            u32x4 flag;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned w = vf[j][i];
-                const bool x0 = (w & 0x7f80u) == 0x7f80u, x1 = (w & 0x7f800000u) == 0x7f800000u;
-                flag[i] = (x0 ? 0x3f80u : 0u) | (x1 ? 0x3f800000u : 0u);
-                vf[j][i] = w & ~((x0 ? 0xffffu : 0u) | (x1 ? 0xffff0000u : 0u));
-            }
-            bad[j] = __builtin_bit_cast(bf16x8, flag);
-        }
-    }
+}
+
+// scores -> weights, as operands of the second product; the state follows the new maximum
+template <int NB, int BITS, typename T, int QT>
+__device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2], WaveState<NB, BITS, T, QT>& st, bf16x8 (&pf)[QT][AttnTerms<T>::p], int k0, bool masked,
+                                             const int (&lo)[QT], const int (&hi)[QT], float c, int lane) {
+    constexpr int DV = RawTile<NB, BITS>::DV;
+    const int g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         float x[8];
@@ -291,48 +274,89 @@ __device__ __forceinline__ void tile_step(const RawTile<NB, BITS>& r, WaveState<
             sum += p[i];
         }
         st.l[t] += sum;
-        bf16x8 pf[NP];
-        split_p<NP>(p, pf);
-#pragma unroll
-        for (int n = NP - 1; n >= 0; --n)
-#pragma unroll
-            for (int j = 0; j < DV; ++j)
-                st.acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[j]), pf[n], st.acc[t][j], 0, 0, 0);
-        if constexpr (CAREFUL) {
-            u32x4 seen;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k1 = k0 + v_row(g, 2 * i), k2 = k0 + v_row(g, 2 * i + 1);
-                seen[i] = (k1 <= hi[t] && k1 >= lo[t] ? 0x3f80u : 0u) | (k2 <= hi[t] && k2 >= lo[t] ? 0x3f800000u : 0u);
-            }
-#pragma unroll
-            for (int j = 0; j < DV; ++j) {
-                f32x4 n = {0.f, 0.f, 0.f, 0.f};
-                n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bad[j], __builtin_bit_cast(bf16x8, seen), n, 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) st.acc[t][j][i] = n[i] > 0.f ? __builtin_nanf("") : st.acc[t][j][i];
-            }
-        }
+        split_p(p, pf[t]);
     }
 }
 
-// the fresh row of position `pos` in place of what the cache still holds there
-template <int NB, int BITS>
-__device__ __forceinline__ void take_fresh(RawTile<NB, BITS>& r, const unsigned char* fresh, int k0, int pos, int lane) {
-    constexpr int RB = 4 * NB * BITS, KB = RB / 4, DV = RawTile<NB, BITS>::DV, VB = DV * BITS / 8, KW = RawTile<NB, BITS>::KW, VW = RawTile<NB, BITS>::VW;
-    const int li = lane & 15, g = lane >> 4;
-    unsigned kw[KW], vw[VW];
+// acc += V^T P^T, two operands (the even and the odd numbers of a pair) at a time
+template <int NB, int BITS, typename T, int QT>
+__device__ __forceinline__ void tile_values(const RawTile<NB, BITS>& r, WaveState<NB, BITS, T, QT>& st, const bf16x8 (&pf)[QT][AttnTerms<T>::p], int lane) {
+    constexpr int NP = AttnTerms<T>::p, DV = RawTile<NB, BITS>::DV;
+    const int li = lane & 15;
+    float sc[8];
 #pragma unroll
-    for (int i = 0; i < KW; ++i) kw[i] = *(const unsigned*)(fresh + g * KB + 4 * i);
-    load_part<VB>(fresh + RB + (NB == 3 ? min(li, 11) : li) * VB, vw);
-    const unsigned ks = *(const unsigned*)(fresh + 2 * RB), vs = *(const unsigned*)(fresh + 2 * RB + 4);
+    for (int i = 0; i < 8; ++i) sc[i] = scale_of(r.vs[i], NB == 1 ? 0 : NB == 2 ? li >> 3 : li >> 2);
+#pragma unroll
+    for (int j = 0; j < DV / 2; ++j) {
+        u32x4 vf[2];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const unsigned a = decode_pair<BITS>(r.v[i], j, sc[i]), b = decode_pair<BITS>(r.v[i + 1], j, sc[i + 1]);
+            vf[0][i >> 1] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+            vf[1][i >> 1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+                for (int o = 0; o < 2; ++o)
+                    st.acc[t][2 * j + o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[o]), pf[t][n], st.acc[t][2 * j + o], 0, 0, 0);
+    }
+}
+
+// value rows whose block is not finite: zeros in their place, and NaN as the mark of the columns that see one
+template <int NB, int BITS, typename T, int QT>
+__device__ __forceinline__ void clean_values(RawTile<NB, BITS>& r, float (&mark)[QT], int k0, const int (&lo)[QT], const int (&hi)[QT], int lane) {
+    constexpr int VW = RawTile<NB, BITS>::VW;
+    const int li = lane & 15, g = lane >> 4;
+    const int acc_block = NB == 1 ? 0 : NB == 2 ? g >> 1 : g, own_block = NB == 1 ? 0 : NB == 2 ? li >> 3 : li >> 2;
+    unsigned part = 0;                                             // byte b, bit i: row v_row(g, i) is not finite in block b
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) part |= (((r.vs[i] >> (8 * b)) & 255u) >= 228u ? 1u : 0u) << (8 * b + i);
+    unsigned rows = 0;                                             // bit k: key k0 + k is not finite in the block of this lane's accumulators
+#pragma unroll
+    for (int gg = 0; gg < 4; ++gg) {
+        const unsigned m = (unsigned)__builtin_amdgcn_readlane((int)part, 16 * gg) >> (8 * acc_block) & 255u;
+        rows |= (m & 15u) << (4 * gg) | (m >> 4) << (16 + 4 * gg);
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int first = max(lo[t] - k0, 0), last = min(hi[t] - k0, 31);
+        const unsigned seen = first <= last ? (~0u >> (31 - last)) & (~0u << first) : 0u;
+        if (rows & seen) mark[t] = __builtin_nanf("");
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (((r.vs[i] >> (8 * own_block)) & 255u) >= 228u) {
+            r.vs[i] = 0;
+#pragma unroll
+            for (int w = 0; w < VW; ++w) r.v[i][w] = 0;
+        }
+}
+
+// the fresh row (codes of key and value, then their scale words) in place of what the cache still holds at its position
+template <int NB, int BITS>
+__device__ __forceinline__ void take_fresh_key(RawTile<NB, BITS>& r, const unsigned char* fresh, int k0, int pos, int lane) {
+    constexpr int RB = 4 * NB * BITS, KB = RB / 4, KW = RawTile<NB, BITS>::KW;
+    const int li = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const bool here = k0 + li + 16 * h == pos;
 #pragma unroll
-        for (int i = 0; i < KW; ++i) r.k[h][i] = here ? kw[i] : r.k[h][i];
-        r.ks[h] = here ? ks : r.ks[h];
+        for (int i = 0; i < KW; ++i) r.k[h][i] = here ? *(const unsigned*)(fresh + g * KB + 4 * i) : r.k[h][i];
+        r.ks[h] = here ? *(const unsigned*)(fresh + 2 * RB) : r.ks[h];
     }
+}
+template <int NB, int BITS>
+__device__ __forceinline__ void take_fresh_value(RawTile<NB, BITS>& r, const unsigned char* fresh, int k0, int pos, int lane) {
+    constexpr int RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, VB = DV * BITS / 8, VW = RawTile<NB, BITS>::VW;
+    const int li = lane & 15, g = lane >> 4;
+    unsigned vw[VW];
+    lds_words<VB>(fresh + RB + (NB == 3 ? min(li, 11) : li) * VB, vw);
+    const unsigned vs = *(const unsigned*)(fresh + 2 * RB + 4);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const bool here = k0 + v_row(g, i) == pos;
@@ -347,7 +371,7 @@ __device__ __forceinline__ void take_fresh(RawTile<NB, BITS>& r, const unsigned 
 // group, four (row, head) pairs.  (row, head) runs fastest over the workgroups, so that the column groups of one pair meet in
 // one XCD's L2; the last column groups, which see the most keys under a causal mask, start first.
 template <int NB, int BITS, typename T, int QT>
-__global__ __launch_bounds__(256) void attn_cache_kernel(AttnCacheArgs a) {
+__global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnCacheArgs a) {
     constexpr int D = 32 * NB, RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, NQ = AttnTerms<T>::q;
     constexpr int MROW = D + 4;                                    // padded row of the merge buffer
     __shared__ __attribute__((aligned(16))) unsigned char fresh_rows[4][2 * RB + 16];
@@ -456,47 +480,55 @@ __global__ __launch_bounds__(256) void attn_cache_kernel(AttnCacheArgs a) {
         }
     }
 
-    TileSource<NB, BITS> src;
+    TileSource src;
     {
         const long e = max(r.e, 0);
-        src.kc = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
-        src.vc = src.kc + a.g.ckv;
-        src.ksc = a.g.scales + e * a.g.se + (long)h * a.g.sh;
-        src.vsc = src.ksc + a.g.skv;
+        src.k = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
+        src.v = src.k + a.g.ckv;
+        src.ks = a.g.scales + e * a.g.se + (long)h * a.g.sh;
+        src.vs = src.ks + a.g.skv;
     }
     WaveState<NB, BITS, T, QT> st;
     const int first = start + (a.kw == 4 ? 32 * w : 0), stride = a.kw * 32;
-    auto load = [&](RawTile<NB, BITS>& raw, int k0) {
-        if (k0 + 32 <= stop) load_tile<NB, BITS, false>(raw, src, k0, 32, lane);
-        else load_tile<NB, BITS, true>(raw, src, k0, stop - k0, lane);
-        if (fresh_pos >= k0 && fresh_pos < k0 + 32) take_fresh<NB, BITS>(raw, fr, k0, fresh_pos, lane);
+    // one tile's registers: the next keys are requested once the scores stand, the next values once the second product has read its own
+    RawTile<NB, BITS> raw;
+    auto keys = [&](int k0) {
+        load_keys<NB, BITS>(raw, src, k0, stop - k0, lane);
+        if (fresh_pos >= k0 && fresh_pos < k0 + 32) take_fresh_key<NB, BITS>(raw, fr, k0, fresh_pos, lane);
     };
-    auto walk = [&](auto careful) {
-        st.reset();
-        if (first >= stop) return;
-        RawTile<NB, BITS> cur, nxt;
-        load(cur, first);
-        for (int k0 = first; k0 < stop; k0 += stride) {
-            const bool more = k0 + stride < stop;
-            if (more) load(nxt, k0 + stride);
-            const bool masked = decltype(careful)::value || k0 + 31 > kr.hi_all || k0 + 31 >= stop || k0 < kr.lo_all;
-            tile_step<NB, BITS, T, QT, decltype(careful)::value>(cur, st, qf, k0, masked, lo, hi, a.c, lane);
-            if (more) cur = nxt;
+    auto values = [&](int k0) {
+        load_values<NB, BITS>(raw, src, k0, stop - k0, lane);
+        if (fresh_pos >= k0 && fresh_pos < k0 + 32) take_fresh_value<NB, BITS>(raw, fr, k0, fresh_pos, lane);
+    };
+    st.reset();
+    float mark[QT] = {};
+    if (first < stop) {
+        keys(first);
+        values(first);
+    }
+    for (int k0 = first; k0 < stop; k0 += stride) {
+        const bool more = k0 + stride < stop;
+        const bool masked = k0 + 31 > kr.hi_all || k0 + 31 >= stop || k0 < kr.lo_all;
+        f32x4 s[QT][2];
+        bf16x8 pf[QT][AttnTerms<T>::p];
+        tile_scores<NB, BITS, T, QT>(raw, qf, s, lane);
+        if (more) keys(k0 + stride);
+        tile_weights<NB, BITS, T, QT>(s, st, pf, k0, masked, lo, hi, a.c, lane);
+        unsigned suspect = 0;
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) suspect |= raw.vs[i] & (raw.vs[i] << 1) & (raw.vs[i] << 2) & 0x80808080u;
         }
-    };
-    walk(std::integral_constant<bool, false>{});
-    {
-        float z = 0.f;
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-            for (int j = 0; j < DV; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) z = __builtin_fmaf(st.acc[t][j][e], 0.f, z);
-        if (__any(!(z == 0.f))) walk(std::integral_constant<bool, true>{});
+        if (__any(suspect != 0)) clean_values<NB, BITS, T, QT>(raw, mark, k0, lo, hi, lane);
+        tile_values<NB, BITS, T, QT>(raw, st, pf, lane);
+        if (more) values(k0 + stride);
     }
 #pragma unroll
-    for (int t = 0; t < QT; ++t) st.l[t] = rows_sum(st.l[t]);
+    for (int t = 0; t < QT; ++t) {
+        st.l[t] = rows_sum(st.l[t]);
+#pragma unroll
+        for (int j = 0; j < DV; ++j) st.acc[t][j] += mark[t];
+    }
 
     const long part_row = ((long)sp * U + u) * a.N;
     if (a.kw == 1) {                                               // the lane holds numbers 4 DV g .. + 4 DV - 1 of its column
