@@ -611,44 +611,65 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
     }
 }
 
-// the splits of one column put together: one wave a column, D / 64 (rounded up) numbers a lane
-template <typename T>
-__global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, int D, int cols_per_group) {
-    const int lane = threadIdx.x & 63;
-    const long item = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+// The splits of one column put together.  A workgroup takes one column; D / 4 lanes read one split's numbers, so 8 to 32 splits
+// are in flight at a time (read one after the other by one wave, 32 splits cost 15 us of memory round trips, now 4.x).
+template <typename T, int NB>
+__global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, int cols_per_group) {
+    constexpr int D = 32 * NB, LPS = D / 4, PAR = 256 / LPS;       // lanes per split, splits at a time
+    __shared__ float red[4];
+    __shared__ __attribute__((aligned(16))) f32x4 sums[PAR][LPS];
+    __shared__ float ls[PAR];
     const int U = a.g.n * a.g.H;
-    if (item >= (long)U * a.N) return;
-    const int u = (int)(item / a.N), c = (int)(item - (long)u * a.N);
+    const int u = blockIdx.x / a.N, c = blockIdx.x - u * a.N;
     const int i = u / a.g.H, h = u - i * a.g.H, step = c / a.G, hq = h * a.G + c - step * a.G;
     const KvRow r = kv_row(a.g, i);
     const int c0 = c / cols_per_group * cols_per_group;
     const KeyRange kr = key_range(a, r, c0, min(c0 + cols_per_group, a.N) - 1);
     const KeyRange own = key_range(a, r, c, c);
-    const bool none = own.beg >= own.end;
-    const int span = kr.end - (kr.beg & ~31);
-    const int ns = max((span + a.chunk - 1) / a.chunk, 1);
+    const int ns = max((kr.end - (kr.beg & ~31) + a.chunk - 1) / a.chunk, 1);       // splits that this column's group really has
     const long hop = (long)U * a.N * (D + 2);
     const float* base = a.part + ((long)u * a.N + c) * (D + 2);
+    const int tid = threadIdx.x, q = tid % LPS, w = tid / LPS;
     float m = -INFINITY;
-    for (int s = lane; s < ns; s += 64) m = fmaxf(m, base[s * hop + D]);
+    for (int s = tid; s < ns; s += 256) m = fmaxf(m, base[s * hop + D]);
     m = wave_max(m);
-    float l = 0.f, o0 = 0.f, o1 = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < ns; ++s) {
-        const float* y = base + s * hop;
-        const float ms = y[D], f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ms - m) * a.c);
-        l += y[D + 1] * f;
-        if (2 * lane < D) {
-            const f32x2 v = *(const f32x2*)(y + 2 * lane);
-            o0 += v[0] * f;
-            o1 += v[1] * f;
+    if ((tid & 63) == 0) red[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (w < PAR)
+        for (int s = w; s < ns; s += PAR) {
+            const float* y = base + s * hop;
+            const f32x2 v0 = *(const f32x2*)(y + 4 * q), v1 = *(const f32x2*)(y + 4 * q + 2), ml = *(const f32x2*)(y + D);
+            const float f = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ml[0] - m) * a.c);
+            l += ml[1] * f;
+            o += (f32x4){v0[0], v0[1], v1[0], v1[1]} * f;
         }
+    if (w < PAR) {
+        sums[w][q] = o;
+        if (q == 0) ls[w] = l;
     }
-    if (2 * lane >= D) return;
+    __syncthreads();
+    if (tid >= LPS) return;
+    const int parts = min(PAR, ns);
+    o = sums[0][tid];
+    l = ls[0];
+    for (int k = 1; k < parts; ++k) {                              // fixed order
+        o += sums[k][tid];
+        l += ls[k];
+    }
+    const bool none = own.beg >= own.end;
     const float inv = 1.0f / l;
-    T* y = (T*)a.out.p + (long)i * a.out.row + (long)step * a.out.step + (long)hq * a.out.head + 2 * lane;
-    y[0] = (T)(none ? 0.f : o0 * inv);
-    y[1] = (T)(none ? 0.f : o1 * inv);
+    T* y = (T*)a.out.p + (long)i * a.out.row + (long)step * a.out.step + (long)hq * a.out.head + 4 * tid;
+    if constexpr (sizeof(T) == 4) {
+        *(f32x4*)y = none ? (f32x4){0.f, 0.f, 0.f, 0.f} : o * inv;
+    } else {
+        typename Half16<T>::v4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.f : o[e] * inv);
+        *(typename Half16<T>::v4*)y = v;
+    }
 }
 
 template <int NB, int BITS, typename T>
@@ -671,8 +692,11 @@ template <typename T> int otter_attn_cache_launch(const AttnCacheArgs& a, int nb
     else launch_nb<T, 8>(a, nb, qt, blocks, s);
     OTTER_CHECK_LAUNCH("otter_attn_cache");
     if (a.nsplit > 1) {
-        const long items = (long)a.g.n * a.g.H * a.N;
-        hipLaunchKernelGGL(attn_cache_join_kernel<T>, dim3((unsigned)((items + 3) / 4)), dim3(256), 0, s, a, 32 * nb, 16 * qt);
+        const dim3 grid((unsigned)(a.g.n * a.g.H * a.N));           // (bounded with the launch's own grid: columns <= 32 per group and item)
+        if (nb == 1) hipLaunchKernelGGL((attn_cache_join_kernel<T, 1>), grid, dim3(256), 0, s, a, 16 * qt);
+        else if (nb == 2) hipLaunchKernelGGL((attn_cache_join_kernel<T, 2>), grid, dim3(256), 0, s, a, 16 * qt);
+        else if (nb == 3) hipLaunchKernelGGL((attn_cache_join_kernel<T, 3>), grid, dim3(256), 0, s, a, 16 * qt);
+        else hipLaunchKernelGGL((attn_cache_join_kernel<T, 4>), grid, dim3(256), 0, s, a, 16 * qt);
         OTTER_CHECK_LAUNCH("otter_attn_cache (join)");
     }
     return OTTER_OK;

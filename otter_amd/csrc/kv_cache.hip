@@ -1,41 +1,65 @@
 // Writing the quantised K/V cache and reading it back (layout and arithmetic: kv_cache.hpp).
+#include <algorithm>
+
 #include "kv_cache.hpp"
 
 namespace {
 
-// Both kernels move 8 numbers a lane: a lane's codes are 4 (or 8) bytes, four lanes share a block and its scale.  Lanes run
-// along the head dimension, then along the steps, then along the heads: a cache row is contiguous with the row of the next
-// step, so a wave's codes form one run of 256 (512) bytes or more, and its numbers runs of head_dim elements.
-// Memory-bound: head_dim * (element size + BITS / 8) + 4 bytes a row, no reuse.
-template <int NB, int BITS, typename T>
+// Both kernels move 8 numbers a lane and piece: a lane's codes are 4 (or 8) bytes, four lanes share a block and its scale.  Lanes
+// run along the head dimension (a row takes 4, 8 or 16 lanes; with head_dim 96 four of the 16 idle), then along the steps, then
+// along the heads: a cache row is contiguous with the row of the next step, so a wave's codes form one run, and its numbers runs
+// of head_dim elements.  Memory-bound: head_dim * (element size + BITS / 8) + 4 bytes a row, no reuse; a lane takes up to four
+// pieces whose loads are requested together, and the four scale bytes of a row leave in one store.
+template <int NB> struct RowLanes { static constexpr int P = NB == 1 ? 4 : NB == 2 ? 8 : 16, live = 4 * NB; };
+
+template <int NB, int BITS, typename T, int M>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvGeom g, KvOperand<const T> k, KvOperand<const T> v, int vec) {
-    constexpr int P = 4 * NB, RB = 4 * NB * BITS;                   // lanes and bytes per row
-    const int id = blockIdx.x * 256 + threadIdx.x;
-    const int unit = id / P, p = id % P;                            // P divides a quad evenly: a block's four lanes are neighbours
-    const int h = unit / g.T, t = unit - h * g.T;
+    constexpr int P = RowLanes<NB>::P, RB = 4 * NB * BITS;
     const int kv = blockIdx.y;
+    const KvOperand<const T>& o = kv ? v : k;
+    const int p = threadIdx.x % P;
     for (int i = blockIdx.z; i < g.n; i += gridDim.z) {
         const KvRow r = kv_row(g, i);
-        const int at = r.pos + t;
-        bool live = h < g.H && r.e >= 0 && t < r.cnt && at >= 0 && at < g.S;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) {
-            const KvOperand<const T>& o = kv ? v : k;
-            kv_load8<T>(o.p + (long)i * o.row + (long)t * o.step + (long)h * o.head + 8 * p, vec, x);
+        float x[M][8];
+        int h[M], at[M];
+        bool live[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const int unit = (blockIdx.x * M + m) * (256 / P) + (int)threadIdx.x / P;
+            h[m] = unit / g.T;
+            const int t = unit - h[m] * g.T;
+            at[m] = r.pos + t;
+            live[m] = p < RowLanes<NB>::live && h[m] < g.H && r.e >= 0 && t < r.cnt && at[m] >= 0 && at[m] < g.S;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[m][e] = 0.f;
+            if (live[m]) kv_load8<T>(o.p + (long)i * o.row + (long)t * o.step + (long)h[m] * o.head + 8 * p, vec, x[m]);
         }
-        if (g.idx && r.e >= 0 && i + 1 < g.n) {                                    // an episode listed twice: the last listing is the one that is written
+        if (g.idx && r.e >= 0 && i + 1 < g.n) {                     // an episode listed twice: the last listing is the one that is written
             bool later = false;
             for (int j = i + 1 + (int)threadIdx.x; j < g.n; j += 256) later |= g.idx[j] == r.e;
             if (__syncthreads_or(later)) continue;
         }
-        const unsigned sb = kv_scale_byte<BITS>(kv_block_top(x));
-        unsigned w[BITS / 4];
-        kv_encode8<BITS>(x, sb, w);
-        if (live) {
-            unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h * g.ch + (long)at * RB + p * BITS;
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const unsigned sb = kv_scale_byte<BITS>(kv_block_top(x[m]));
+            unsigned w[BITS / 4];
+            kv_encode8<BITS>(x[m], sb, w);
+            unsigned word = sb;                                     // the row's scale bytes, gathered in its first lane
+            if constexpr (NB >= 2) word |= __shfl_down(sb, 4, P) << 8;
+            if constexpr (NB >= 3) word |= __shfl_down(sb, 8, P) << 16;
+            if constexpr (NB >= 4) word |= __shfl_down(sb, 12, P) << 24;
+            if (!live[m]) continue;
+            unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h[m] * g.ch + (long)at[m] * RB + p * BITS;
             if constexpr (BITS == 4) *(unsigned*)c = w[0];
             else *(uint2*)c = make_uint2(w[0], w[1]);
-            if ((p & 3) == 0) g.scales[kv * g.skv + (long)r.e * g.se + (long)h * g.sh + (long)at * 4 + (p >> 2)] = (unsigned char)sb;
+            if (p != 0) continue;
+            unsigned char* sc = g.scales + kv * g.skv + (long)r.e * g.se + (long)h[m] * g.sh + (long)at[m] * 4;
+            if constexpr (NB == 1) *sc = (unsigned char)word;
+            else if constexpr (NB == 4) *(unsigned*)sc = word;
+            else {
+                *(unsigned short*)sc = (unsigned short)word;
+                if constexpr (NB == 3) sc[2] = (unsigned char)(word >> 16);
+            }
         }
     }
 }
@@ -79,28 +103,40 @@ template <typename T> __device__ __forceinline__ void kv_store8(T* p, bool vec, 
     }
 }
 
-template <int NB, int BITS, typename T>
+template <int NB, int BITS, typename T, int M>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvGeom g, KvOperand<T> k, KvOperand<T> v, int vec) {
-    constexpr int P = 4 * NB, RB = 4 * NB * BITS;
-    const int id = blockIdx.x * 256 + threadIdx.x;
-    const int unit = id / P, p = id % P;
-    const int h = unit / g.T, t = unit - h * g.T;
-    if (h >= g.H) return;
+    constexpr int P = RowLanes<NB>::P, RB = 4 * NB * BITS;
     const int kv = blockIdx.y;
+    const KvOperand<T>& o = kv ? v : k;
+    const int p = threadIdx.x % P;
+    if (p >= RowLanes<NB>::live) return;
     for (int i = blockIdx.z; i < g.n; i += gridDim.z) {
         const KvRow r = kv_row(g, i);
-        const int at = r.pos + t;
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (r.e >= 0 && t < r.cnt && at >= 0 && at < g.S) {
-            const unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h * g.ch + (long)at * RB + p * BITS;
-            const unsigned sb = g.scales[kv * g.skv + (long)r.e * g.se + (long)h * g.sh + (long)at * 4 + (p >> 2)];
-            unsigned w[BITS / 4];
-            if constexpr (BITS == 4) w[0] = *(const unsigned*)c;
-            else { const uint2 u = *(const uint2*)c; w[0] = u.x; w[1] = u.y; }
-            kv_decode8<BITS>(w, sb, x);
+        unsigned w[M][BITS / 4], sb[M];
+        int h[M], t[M];
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            const int unit = (blockIdx.x * M + m) * (256 / P) + (int)threadIdx.x / P;
+            h[m] = unit / g.T;
+            t[m] = unit - h[m] * g.T;
+            const int at = r.pos + t[m];
+            sb[m] = 0;
+#pragma unroll
+            for (int q = 0; q < BITS / 4; ++q) w[m][q] = 0;
+            if (h[m] < g.H && r.e >= 0 && t[m] < r.cnt && at >= 0 && at < g.S) {
+                const unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h[m] * g.ch + (long)at * RB + p * BITS;
+                sb[m] = g.scales[kv * g.skv + (long)r.e * g.se + (long)h[m] * g.sh + (long)at * 4 + (p >> 2)];
+                if constexpr (BITS == 4) w[m][0] = *(const unsigned*)c;
+                else { const uint2 u = *(const uint2*)c; w[m][0] = u.x; w[m][1] = u.y; }
+            }
         }
-        const KvOperand<T>& o = kv ? v : k;
-        kv_store8<T>(o.p + (long)i * o.row + (long)t * o.step + (long)h * o.head + 8 * p, vec, x);
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            if (h[m] >= g.H) continue;
+            float x[8];
+            kv_decode8<BITS>(w[m], sb[m], x);                       // (what does not exist: codes 0, the number 0)
+            kv_store8<T>(o.p + (long)i * o.row + (long)t[m] * o.step + (long)h[m] * o.head + 8 * p, vec, x);
+        }
     }
 }
 
@@ -109,16 +145,23 @@ inline bool operand_vec(const otter_kv_operand* o, int dtype) {
     return aligned16(o->p) && (o->row * es) % 16 == 0 && (o->step * es) % 16 == 0 && (o->head * es) % 16 == 0;
 }
 
-template <bool WRITE, int NB, int BITS, typename T>
-void launch(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
-    const long lanes = (long)g.H * g.T * 4 * NB;
-    const dim3 grid((unsigned)((lanes + 255) / 256), 2, (unsigned)min(g.n, 65535));
+template <bool WRITE, int NB, int BITS, typename T, int M>
+void launch_m(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
+    const long rows = (long)g.H * g.T, a_block = M * (256 / RowLanes<NB>::P);
+    const dim3 grid((unsigned)((rows + a_block - 1) / a_block), 2, (unsigned)std::min(g.n, 65535));
     if constexpr (WRITE)
-        hipLaunchKernelGGL((kv_write_kernel<NB, BITS, T>), grid, dim3(256), 0, s, g, (KvOperand<const T>{(const T*)k->p, k->row, k->step, k->head}),
+        hipLaunchKernelGGL((kv_write_kernel<NB, BITS, T, M>), grid, dim3(256), 0, s, g, (KvOperand<const T>{(const T*)k->p, k->row, k->step, k->head}),
                            (KvOperand<const T>{(const T*)v->p, v->row, v->step, v->head}), vec);
     else
-        hipLaunchKernelGGL((kv_read_kernel<NB, BITS, T>), grid, dim3(256), 0, s, g, (KvOperand<T>{(T*)k->p, k->row, k->step, k->head}),
+        hipLaunchKernelGGL((kv_read_kernel<NB, BITS, T, M>), grid, dim3(256), 0, s, g, (KvOperand<T>{(T*)k->p, k->row, k->step, k->head}),
                            (KvOperand<T>{(T*)v->p, v->row, v->step, v->head}), vec);
+}
+
+// one piece a lane while that leaves the chip short of workgroups, four otherwise
+template <bool WRITE, int NB, int BITS, typename T>
+void launch(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
+    if ((long)g.H * g.T * RowLanes<NB>::P / 1024 * 2 * g.n >= 2048) launch_m<WRITE, NB, BITS, T, 4>(g, k, v, vec, s);
+    else launch_m<WRITE, NB, BITS, T, 1>(g, k, v, vec, s);
 }
 
 template <bool WRITE, int BITS, typename T>
@@ -135,7 +178,7 @@ int move(const otter_kv_cache* c, const otter_kv_rows* r, int dtype, const otter
     if (r->n_rows == 0 || r->steps == 0) return OTTER_OK;
     if (int rc = otter_kv_check_operand(k, dtype, !WRITE, "k", name)) return rc;
     if (int rc = otter_kv_check_operand(v, dtype, !WRITE, "v", name)) return rc;
-    OTTER_REQUIRE((long)c->heads * r->steps * (c->head_dim / 8) < (1L << 31) - 256, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: %d heads x %d steps too large", name, c->heads, r->steps);
+    OTTER_REQUIRE((long)c->heads * r->steps * 16 < (1L << 31) - 1024, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: %d heads x %d steps too large", name, c->heads, r->steps);
     const KvGeom g = otter_kv_geom(c, r);
     const int vec = operand_vec(k, dtype) && operand_vec(v, dtype), nb = c->head_dim / 32;
     if (c->bits == 4) {
