@@ -5,29 +5,33 @@
 
 namespace {
 
-struct Plan { int qt, cg, kw, nsplit, chunk; unsigned blocks; bool ok; };
+struct Plan { int qt, wide, cg, kw, nsplit, chunk; unsigned blocks; bool ok; };
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-// Columns: 16 per wave while all of a row's columns fit, 32 otherwise.  Keys: one wave walks over all of them while there are
-// enough waves to fill the chip, four waves (and several workgroups) share them otherwise.
-Plan plan(int n, int H, int N, int G, int window, int max_len) {
+// Columns: 16 per wave while all of a row's columns fit, then 32; from 33 on, with several steps, four waves share the
+// converted tiles.
+// Keys: one wave (wide: one workgroup) walks over all of them while there are enough to fill the chip, four waves and several
+// workgroups share them otherwise.
+Plan plan(int n, int H, int steps, int G, int window, int max_len) {
     Plan p{};
-    const long U = (long)n * H;
-    p.qt = N <= 16 ? 1 : 2;
-    p.cg = (int)ceil_div(N, 16 * p.qt);
-    const long span = (window > 0 ? std::min<long>(max_len, (long)window + (16L * p.qt) / G + 1) : max_len) + 31;   // keys one item may walk over
+    const long U = (long)n * H, N = (long)steps * G;
+    p.wide = N > 32 && steps > 1;
+    p.qt = N <= 16 || (p.wide && N <= 64) ? 1 : 2;
+    const long cols = (p.wide ? 64L : 16L) * p.qt;
+    p.cg = (int)ceil_div(N, cols);
+    const long span = (window > 0 ? std::min<long>(max_len, (long)window + cols / G + 1) : max_len) + 31;   // keys one item may walk over
     const long items = U * p.cg;
-    p.kw = (span > 95 && items < 4096) ? 4 : 1;
+    p.kw = (!p.wide && span > 95 && items < 4096) ? 4 : 1;
     p.nsplit = 1;
     p.chunk = (int)(ceil_div(span, 128) * 128);
-    if (p.kw == 4) {
-        const long want = ceil_div(1024, items), most = ceil_div(span, 256);
+    if (p.kw == 4 || (p.wide && items < 512)) {
+        const long want = ceil_div(p.wide ? 512 : 1024, items), most = ceil_div(span, p.wide ? 512 : 256);
         const long ns = std::max<long>(1, std::min(want, most));
         p.chunk = (int)(ceil_div(ceil_div(span, ns), 128) * 128);
         p.nsplit = (int)ceil_div(span, p.chunk);
     }
-    const long blocks = p.kw == 4 ? items * p.nsplit : p.cg == 1 ? ceil_div(U, 4) : U * ceil_div(p.cg, 4);
+    const long blocks = p.wide || p.kw == 4 ? items * p.nsplit : p.cg == 1 ? ceil_div(U, 4) : U * ceil_div(p.cg, 4);
     p.ok = blocks < (1L << 31);
     p.blocks = (unsigned)blocks;
     return p;
@@ -38,7 +42,7 @@ Plan plan(int n, int H, int N, int G, int window, int max_len) {
 extern "C" long otter_attn_cache_workspace_floats(int n_rows, int steps, int q_heads, int kv_heads, int head_dim, int window, int max_len) {
     if (n_rows <= 0 || steps <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 || max_len <= 0 || window < 0) return 0;
     if ((long)steps * (q_heads / kv_heads) >= (1L << 31) || (long)n_rows * kv_heads >= (1L << 31)) return 0;
-    const Plan p = plan(n_rows, kv_heads, steps * (q_heads / kv_heads), q_heads / kv_heads, window, max_len);
+    const Plan p = plan(n_rows, kv_heads, steps, q_heads / kv_heads, window, max_len);
     return p.nsplit > 1 ? (long)p.nsplit * n_rows * q_heads * steps * (head_dim + 2) : 0;
 }
 
@@ -66,7 +70,7 @@ extern "C" int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows
     const int G = q_heads / cache->heads;
     OTTER_REQUIRE((long)rows->steps * G < (1L << 30) && (long)rows->n_rows * cache->heads < (1L << 30), OTTER_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, heads or steps", name);
     const int cap = std::min(max_len, cache->capacity);
-    Plan p = plan(rows->n_rows, cache->heads, rows->steps * G, G, window, cap);
+    Plan p = plan(rows->n_rows, cache->heads, rows->steps, G, window, cap);
     OTTER_REQUIRE(p.ok, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", name);
     if (p.nsplit > 1) {
         const long need = (long)p.nsplit * rows->n_rows * q_heads * rows->steps * (cache->head_dim + 2);
@@ -90,6 +94,7 @@ extern "C" int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows
     a.window = window;
     a.max_len = cap;
     a.c = scale * 1.44269504088896341f;
+    a.wide = p.wide;
     a.kw = p.kw;
     a.nsplit = p.nsplit;
     a.chunk = p.chunk;

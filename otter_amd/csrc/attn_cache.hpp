@@ -25,9 +25,10 @@ struct AttnCacheArgs {
     KvOperand<const void> q; int q_vec;
     KvOperand<void> out;
     KvOperand<const void> kn, vn; int new_vec;      // fresh key / value rows to append (null: the cache is complete)
-    int G, N, CG;                                   // query heads per key head, columns T * G, column groups of 16 * QT
+    int G, N, CG;                                   // query heads per key head, columns T * G, column groups of 16 * QT (64 * QT: wide)
     int causal, window, max_len;
     float c;
+    int wide;                                       // 1: four waves x 16 QT columns a workgroup over tiles that they convert together
     int kw, nsplit, chunk;                          // waves per item along the keys (1 or 4), splits of the key range, keys per split (multiple of 32 * kw)
     float* part;                                    // [nsplit][n * H][N][D + 2] partial sums: D numbers, maximum, sum
 };
@@ -237,25 +238,34 @@ __device__ __forceinline__ void tile_scores(const RawTile<NB, BITS>& r, const bf
     }
 }
 
-// scores -> weights, as operands of the second product; the state follows the new maximum
-template <int NB, int BITS, typename T, int QT>
-__device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2], WaveState<NB, BITS, T, QT>& st, bf16x8 (&pf)[QT][AttnTerms<T>::p], int k0, bool masked,
-                                             const int (&lo)[QT], const int (&hi)[QT], float c, int lane) {
+// scores of NS x 32 keys -> weights, as operands of the second product; the state follows the new maximum
+template <int NB, int BITS, typename T, int QT, int NS>
+__device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2 * NS], WaveState<NB, BITS, T, QT>& st, bf16x8 (&pf)[NS][QT][AttnTerms<T>::p], int k0,
+                                             bool masked, const int (&lo)[QT], const int (&hi)[QT], float c, int lane) {
     constexpr int DV = RawTile<NB, BITS>::DV;
     const int g = lane >> 4;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        float x[8];
+        float x[NS][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = s[t][i >> 2][i & 3];
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[u][i] = s[t][2 * u + (i >> 2)][i & 3];
         if (masked) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int key = k0 + v_row(g, i);
-                x[i] = (key <= hi[t] && key >= lo[t]) ? x[i] : -INFINITY;
-            }
+            for (int u = 0; u < NS; ++u)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = k0 + 32 * u + v_row(g, i);
+                    x[u][i] = (key <= hi[t] && key >= lo[t]) ? x[u][i] : -INFINITY;
+                }
         }
-        float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+        float mx = x[0][0];
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+            const float m4 = fmaxf(fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])), fmaxf(fmaxf(x[u][4], x[u][5]), fmaxf(x[u][6], x[u][7])));
+            mx = u ? fmaxf(mx, m4) : m4;
+        }
         mx = rows_max(mx);
         const float mn = fmaxf(st.m[t], mx);
         const float mc = mn == -INFINITY ? 0.f : mn * c;
@@ -266,15 +276,18 @@ __device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2], WaveState<
             for (int j = 0; j < DV; ++j) st.acc[t][j] *= corr;
         }
         st.m[t] = mn;
-        float p[8];
-        float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], c, -mc));
-            sum += p[i];
+        for (int u = 0; u < NS; ++u) {
+            float p[8];
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], c, -mc));
+                sum += p[i];
+            }
+            st.l[t] += sum;
+            split_p(p, pf[u][t]);
         }
-        st.l[t] += sum;
-        split_p(p, pf[t]);
     }
 }
 
@@ -366,6 +379,81 @@ __device__ __forceinline__ void take_fresh_value(RawTile<NB, BITS>& r, const uns
     }
 }
 
+// the columns of a lane: positions that each sees
+template <int QT> __device__ __forceinline__ void lane_columns(const AttnCacheArgs& a, const KvRow& r, int c0, int li, int (&col)[QT], int (&lo)[QT], int (&hi)[QT]) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        col[t] = c0 + 16 * t + li;
+        const int step = col[t] / a.G;
+        const int qp = a.causal ? r.pos + step : r.pos + r.cnt - 1;
+        hi[t] = (col[t] < a.N && step < r.cnt && r.e >= 0) ? min(min(qp, a.g.S - 1), a.max_len - 1) : -1;
+        lo[t] = a.window ? max(qp - a.window + 1, 0) : 0;
+    }
+}
+
+// query operands: numbers 8 NB g + 8 j .. + 7 of the lane's column, as a sum of bf16 terms (cut, not rounded: the rest is exact)
+template <int NB, typename T, int QT>
+__device__ __forceinline__ void load_queries(const AttnCacheArgs& a, int i, int h, const int (&col)[QT], int g, bf16x8 (&qf)[QT][AttnTerms<T>::q][NB]) {
+    constexpr int NQ = AttnTerms<T>::q;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int step = col[t] / a.G, hq = h * a.G + col[t] - step * a.G;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (col[t] < a.N) kv_load8<T>((const T*)a.q.p + (long)i * a.q.row + (long)step * a.q.step + (long)hq * a.q.head + 8 * (NB * g + j), a.q_vec, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float rest = x[e];
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    const float cut = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
+                    qf[t][n][j][e] = (__bf16)cut;
+                    rest -= cut;
+                }
+            }
+        }
+    }
+}
+
+// a lane's columns: numbers 4 DV g .. + 4 DV - 1, to the output (one split) or, not yet divided, to the scratch
+template <int NB, int BITS, typename T, int QT>
+__device__ __forceinline__ void store_columns(const AttnCacheArgs& a, const WaveState<NB, BITS, T, QT>& st, int u, int i, int h, int sp, const int (&col)[QT],
+                                              const int (&lo)[QT], const int (&hi)[QT], int g) {
+    constexpr int D = 32 * NB, DV = RawTile<NB, BITS>::DV;
+    if (NB == 3 && g == 3) return;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        if (col[t] >= a.N) continue;
+        if (a.nsplit > 1) {
+            float* y = a.part + (((long)sp * a.g.n * a.g.H + u) * a.N + col[t]) * (D + 2);
+#pragma unroll
+            for (int d = 0; d < 4 * DV; d += 2) *(f32x2*)(y + 4 * DV * g + d) = (f32x2){st.acc[t][d % DV][d / DV], st.acc[t][(d + 1) % DV][(d + 1) / DV]};
+            if (g == 0) *(f32x2*)(y + D) = (f32x2){st.m[t], st.l[t]};
+            continue;
+        }
+        const int step = col[t] / a.G, hq = h * a.G + col[t] - step * a.G;
+        const bool none = lo[t] > hi[t];
+        const float inv = 1.0f / st.l[t];
+        T* o = (T*)a.out.p + (long)i * a.out.row + (long)step * a.out.step + (long)hq * a.out.head + 4 * DV * g;
+#pragma unroll
+        for (int q = 0; q < DV / 2; ++q) {                         // 8 consecutive numbers at a time
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { const int d = 8 * q + e; y[e] = none ? 0.f : st.acc[t][d % DV][d / DV] * inv; }
+            if constexpr (sizeof(T) == 4) {
+                *(f32x4*)(o + 8 * q) = (f32x4){y[0], y[1], y[2], y[3]};
+                *(f32x4*)(o + 8 * q + 4) = (f32x4){y[4], y[5], y[6], y[7]};
+            } else {
+                typename Half16<T>::v8 v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = (T)y[e];
+                *(typename Half16<T>::v8*)(o + 8 * q) = v;
+            }
+        }
+    }
+}
+
 // Items: (split, row, key head, column group).  A workgroup of four waves takes one item with the keys dealt out in tiles
 // (kw = 4), or four items: neighbouring column groups of one (row, head), which read the same rows, or, with one column
 // group, four (row, head) pairs.  (row, head) runs fastest over the workgroups, so that the column groups of one pair meet in
@@ -404,16 +492,8 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
     if (sp > 0 && start >= stop) return;                           // the whole workgroup: the item has fewer splits
     const bool whole = a.nsplit == 1;
 
-    // columns of this lane
     int lo[QT], hi[QT], col[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        col[t] = c0 + 16 * t + li;
-        const int step = col[t] / a.G;
-        const int qp = a.causal ? r.pos + step : r.pos + r.cnt - 1;
-        hi[t] = (col[t] < a.N && step < r.cnt && r.e >= 0) ? min(min(qp, a.g.S - 1), a.max_len - 1) : -1;
-        lo[t] = a.window ? max(qp - a.window + 1, 0) : 0;
-    }
+    lane_columns<QT>(a, r, c0, li, col, lo, hi);
 
     // the fresh row: codes to the cache and, for this wave's own tiles, to LDS
     unsigned char* fr = fresh_rows[w];
@@ -458,27 +538,8 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
         __builtin_amdgcn_wave_barrier();
     }
 
-    // query operands: numbers 8 NB g + 8 j .. + 7 of the lane's column, as a sum of bf16 terms (cut, not rounded: the rest is exact)
     bf16x8 qf[QT][NQ][NB];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        const int step = col[t] / a.G, hq = h * a.G + col[t] - step * a.G;
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (col[t] < a.N) kv_load8<T>((const T*)a.q.p + (long)i * a.q.row + (long)step * a.q.step + (long)hq * a.q.head + 8 * (NB * g + j), a.q_vec, x);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                float rest = x[e];
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    const float cut = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-                    qf[t][n][j][e] = (__bf16)cut;
-                    rest -= cut;
-                }
-            }
-        }
-    }
+    load_queries<NB, T, QT>(a, i, h, col, g, qf);
 
     TileSource src;
     {
@@ -510,17 +571,17 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
         const bool more = k0 + stride < stop;
         const bool masked = k0 + 31 > kr.hi_all || k0 + 31 >= stop || k0 < kr.lo_all;
         f32x4 s[QT][2];
-        bf16x8 pf[QT][AttnTerms<T>::p];
+        bf16x8 pf[1][QT][AttnTerms<T>::p];
         tile_scores<NB, BITS, T, QT>(raw, qf, s, lane);
         if (more) keys(k0 + stride);
-        tile_weights<NB, BITS, T, QT>(s, st, pf, k0, masked, lo, hi, a.c, lane);
+        tile_weights<NB, BITS, T, QT, 1>(s, st, pf, k0, masked, lo, hi, a.c, lane);
         unsigned suspect = 0;
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) suspect |= raw.vs[i] & (raw.vs[i] << 1) & (raw.vs[i] << 2) & 0x80808080u;
         }
         if (__any(suspect != 0)) clean_values<NB, BITS, T, QT>(raw, mark, k0, lo, hi, lane);
-        tile_values<NB, BITS, T, QT>(raw, st, pf, lane);
+        tile_values<NB, BITS, T, QT>(raw, st, pf[0], lane);
         if (more) values(k0 + stride);
     }
 #pragma unroll
@@ -531,31 +592,8 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
     }
 
     const long part_row = ((long)sp * U + u) * a.N;
-    if (a.kw == 1) {                                               // the lane holds numbers 4 DV g .. + 4 DV - 1 of its column
-        if (NB == 3 && g == 3) return;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            if (col[t] >= a.N) continue;
-            const int step = col[t] / a.G, hq = h * a.G + col[t] - step * a.G;
-            const float inv = lo[t] <= hi[t] ? 1.0f / st.l[t] : 0.f;
-            T* o = (T*)a.out.p + (long)i * a.out.row + (long)step * a.out.step + (long)hq * a.out.head + 4 * DV * g;
-            const bool none = lo[t] > hi[t];
-#pragma unroll
-            for (int q = 0; q < DV / 2; ++q) {                     // 8 consecutive numbers: rows 8 / DV at a time
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) { const int d = 8 * q + e; y[e] = none ? 0.f : st.acc[t][d % DV][d / DV] * inv; }
-                if constexpr (sizeof(T) == 4) {
-                    *(f32x4*)(o + 8 * q) = (f32x4){y[0], y[1], y[2], y[3]};
-                    *(f32x4*)(o + 8 * q + 4) = (f32x4){y[4], y[5], y[6], y[7]};
-                } else {
-                    typename Half16<T>::v8 v;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = (T)y[e];
-                    *(typename Half16<T>::v8*)(o + 8 * q) = v;
-                }
-            }
-        }
+    if (a.kw == 1) {
+        store_columns<NB, BITS, T, QT>(a, st, u, i, h, sp, col, lo, hi, g);
         return;
     }
     // four waves saw different keys of the same columns: merge through LDS, 16 columns at a time
@@ -609,6 +647,193 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
             }
         }
     }
+}
+
+// ------------------------------------------------------------------------------------------------
+// Many columns a row (whole windows, chunks): a workgroup's four waves own neighbouring column groups of one (row, head) and walk
+// over its keys together.  Converting a tile takes as many vector instructions as a column group's softmax, so the four waves
+// convert 64 keys once between them -- a wave its 16 keys and half the numbers of its 32 value rows -- into LDS, in the order in
+// which the matrix operands are read (16 bytes a lane, no conflicts), while the previous tile is being multiplied: two buffers,
+// one barrier a tile.
+template <int NB, int BITS> struct WideTile {
+    static constexpr int DV = RawTile<NB, BITS>::DV, KW = RawTile<NB, BITS>::KW;
+    static constexpr int PW = DV / 4 > 0 ? DV / 4 : 1;             // pairs of numbers of a value row that one wave converts
+    static constexpr int PB = PW * BITS / 4;                       // bytes of those
+    static constexpr int frags = 4 * NB + 2 * DV;                  // operands of 64 lanes x 16 bytes: 4 x 16 keys, then 2 x 32 value rows
+    static constexpr int bytes = frags * 1024 + 64;                // and a row mask per (32 keys, block) of the value rows that are not finite
+    unsigned k[KW], v[8][1], ks, vs[8];
+};
+
+template <int NB, int BITS> __device__ __forceinline__ void wide_load(WideTile<NB, BITS>& r, const TileSource& src, int k0, int rows, int lane, int w) {
+    constexpr int RB = 4 * NB * BITS, KB = RB / 4, VB = RawTile<NB, BITS>::DV * BITS / 8, PB = WideTile<NB, BITS>::PB;
+    const int li = lane & 15, g = lane >> 4;
+    const auto kc = rows_of(src.k, k0 + 16 * w, RB, rows - 16 * w), ks = rows_of(src.ks, k0 + 16 * w, 4, rows - 16 * w);
+    buffer_words<KB>(kc, li * RB + g * KB, r.k);
+    r.ks = __builtin_amdgcn_raw_buffer_load_b32(ks, li * 4, 0, 0);
+    if (NB == 1 && (w & 1)) return;                                // (one pair a lane: two waves do it)
+    const int sub = 32 * (w >> 1);
+    const auto vc = rows_of(src.v, k0 + sub, RB, rows - sub), vs = rows_of(src.vs, k0 + sub, 4, rows - sub);
+    const int vl = (NB == 3 ? min(li, 11) : li) * VB + (w & 1) * PB + 4 * g * RB;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b128(vs, 16 * g + 64 * h, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.vs[4 * h + i] = u[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) buffer_words<PB>(vc, vl + ((i & 3) + 16 * (i >> 2)) * RB, r.v[i]);
+}
+
+// `edge`: the tile has keys that some column does not see: blocks that are not finite are taken out and named in the masks
+template <int NB, int BITS> __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned char* buf, bool edge, int lane, int w) {
+    typedef WideTile<NB, BITS> W;
+    const int li = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+        *(bf16x8*)(buf + (w * NB + j) * 1024 + lane * 16) =
+            decode8<BITS>(&r.k[j * BITS / 4], scale_of(r.ks, NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2));
+    if (NB == 1 && (w & 1)) return;
+    const int block = NB == 1 ? 0 : NB == 2 ? li >> 3 : li >> 2;
+    if (edge) {
+        unsigned part = 0;                                         // byte b, bit i: row v_row(g, i) is not finite in block b
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) part |= (((r.vs[i] >> (8 * b)) & 255u) >= 228u ? 1u : 0u) << (8 * b + i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (((r.vs[i] >> (8 * block)) & 255u) >= 228u) r.vs[i] = r.v[i][0] = 0;
+        unsigned rows[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            rows[b] = 0;
+#pragma unroll
+            for (int gg = 0; gg < 4; ++gg) {
+                const unsigned m = (unsigned)__builtin_amdgcn_readlane((int)part, 16 * gg) >> (8 * b) & 255u;
+                rows[b] |= (m & 15u) << (4 * gg) | (m >> 4) << (16 + 4 * gg);
+            }
+        }
+        if ((w & 1) == 0 && lane == 0) *(u32x4*)(buf + W::frags * 1024 + 16 * (w >> 1)) = (u32x4){rows[0], rows[1], rows[2], rows[3]};
+    }
+    float sc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sc[i] = scale_of(r.vs[i], block);
+    unsigned char* to = buf + (4 * NB + (w >> 1) * W::DV + (w & 1) * 2 * W::PW) * 1024 + lane * 16;
+#pragma unroll
+    for (int j = 0; j < W::PW; ++j) {
+        u32x4 vf[2];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const unsigned a = decode_pair<BITS>(r.v[i], j, sc[i]), b = decode_pair<BITS>(r.v[i + 1], j, sc[i + 1]);
+            vf[0][i >> 1] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+            vf[1][i >> 1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        }
+        *(u32x4*)(to + 2 * j * 1024) = vf[0];
+        *(u32x4*)(to + (2 * j + 1) * 1024) = vf[1];
+    }
+}
+
+template <int NB, int BITS, typename T, int QT>
+__global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a) {
+    constexpr int DV = RawTile<NB, BITS>::DV, NQ = AttnTerms<T>::q, NP = AttnTerms<T>::p;
+    typedef WideTile<NB, BITS> W;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, g = lane >> 4;
+    const int U = a.g.n * a.g.H;
+    const int u = blockIdx.x % U, rest = blockIdx.x / U;           // (row, head) fastest, then column groups from the last on, then splits
+    const int cg = a.CG - 1 - rest % a.CG, sp = rest / a.CG;
+    const int i = u / a.g.H, h = u - i * a.g.H;
+    const KvRow r = kv_row(a.g, i);
+    const int all0 = cg * 64 * QT, c0 = all0 + w * 16 * QT;
+    const KeyRange kr = key_range(a, r, all0, min(all0 + 64 * QT, a.N) - 1);
+    const int start = (kr.beg & ~31) + sp * a.chunk, stop = min(kr.end, start + a.chunk);
+    if (sp > 0 && start >= stop) return;
+    const KeyRange own = c0 < a.N ? key_range(a, r, c0, min(c0 + 16 * QT, a.N) - 1) : KeyRange{0, 0, -1, 0};
+    int lo[QT], hi[QT], col[QT];
+    lane_columns<QT>(a, r, c0, li, col, lo, hi);
+    bf16x8 qf[QT][NQ][NB];
+    load_queries<NB, T, QT>(a, i, h, col, g, qf);
+    TileSource src;
+    {
+        const long e = max(r.e, 0);
+        src.k = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
+        src.v = src.k + a.g.ckv;
+        src.ks = a.g.scales + e * a.g.se + (long)h * a.g.sh;
+        src.vs = src.ks + a.g.skv;
+    }
+    WaveState<NB, BITS, T, QT> st;
+    st.reset();
+    float mark[QT] = {};
+    auto edge = [&](int k0) { return k0 + 63 > kr.hi_all || k0 + 64 > stop || k0 < kr.lo_all; };
+    WideTile<NB, BITS> raw;
+    if (start < stop) {
+        wide_load<NB, BITS>(raw, src, start, stop - start, lane, w);
+        wide_convert<NB, BITS>(raw, lds, edge(start), lane, w);
+        if (start + 64 < stop) wide_load<NB, BITS>(raw, src, start + 64, stop - start - 64, lane, w);
+    }
+    __syncthreads();
+    int at = 0;
+    for (int k0 = start; k0 < stop; k0 += 64, at ^= 1) {
+        const unsigned char* buf = lds + at * W::bytes;
+        const bool work = k0 < own.end && k0 + 64 > own.beg;       // somebody in this wave sees a key of the tile
+        const bool more = k0 + 64 < stop;
+        bf16x8 pf[2][QT][NP];
+        if (work) {
+            f32x4 s[QT][4];
+#pragma unroll
+            for (int hh = 0; hh < 4; ++hh) {
+#pragma unroll
+                for (int t = 0; t < QT; ++t) s[t][hh] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    const bf16x8 kf = *(const bf16x8*)(buf + (hh * NB + j) * 1024 + lane * 16);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+#pragma unroll
+                        for (int n = NQ - 1; n >= 0; --n) s[t][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][n][j], s[t][hh], 0, 0, 0);
+                }
+            }
+            const bool masked = k0 + 63 > own.hi_all || k0 + 64 > stop || k0 < own.lo_all;
+            tile_weights<NB, BITS, T, QT, 2>(s, st, pf, k0, masked, lo, hi, a.c, lane);
+        }
+        if (more) {                                                // the next tile into the other buffer, the one behind it on its way
+            wide_convert<NB, BITS>(raw, lds + (at ^ 1) * W::bytes, edge(k0 + 64), lane, w);
+            if (k0 + 128 < stop) wide_load<NB, BITS>(raw, src, k0 + 128, stop - k0 - 128, lane, w);
+        }
+        if (work) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int j = 0; j < DV; ++j) {
+                    const bf16x8 vf = *(const bf16x8*)(buf + (4 * NB + x * DV + j) * 1024 + lane * 16);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+#pragma unroll
+                        for (int n = NP - 1; n >= 0; --n) st.acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x][t][n], st.acc[t][j], 0, 0, 0);
+                }
+            if (edge(k0)) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const unsigned rows = *(const unsigned*)(buf + W::frags * 1024 + 16 * x + 4 * (NB == 1 ? 0 : NB == 2 ? g >> 1 : g));
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                        const int first = max(lo[t] - k0 - 32 * x, 0), last = min(hi[t] - k0 - 32 * x, 31);
+                        const unsigned seen = first <= last ? (~0u >> (31 - last)) & (~0u << first) : 0u;
+                        if (rows & seen) mark[t] = __builtin_nanf("");
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        st.l[t] = rows_sum(st.l[t]);
+#pragma unroll
+        for (int j = 0; j < DV; ++j) st.acc[t][j] += mark[t];
+    }
+    store_columns<NB, BITS, T, QT>(a, st, u, i, h, sp, col, lo, hi, g);
 }
 
 // The splits of one column put together.  A workgroup takes one column; D / 4 lanes read one split's numbers, so 8 to 32 splits
@@ -672,31 +897,41 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, i
     }
 }
 
-template <int NB, int BITS, typename T>
-void launch_qt(const AttnCacheArgs& a, int qt, unsigned blocks, hipStream_t s) {
-    if (qt == 1) hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 1>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
+template <int NB, int BITS, typename T, int QT>
+int launch_wide(const AttnCacheArgs& a, unsigned blocks, hipStream_t s) {
+    constexpr int lds = 2 * WideTile<NB, BITS>::bytes;
+    if (int rc = otter_reserve_lds((const void*)attn_cache_wide_kernel<NB, BITS, T, QT>, lds, "otter_attn_cache")) return rc;
+    hipLaunchKernelGGL((attn_cache_wide_kernel<NB, BITS, T, QT>), dim3(blocks), dim3(256), lds, s, a);
+    return OTTER_OK;
 }
 
-template <typename T, int BITS> void launch_nb(const AttnCacheArgs& a, int nb, int qt, unsigned blocks, hipStream_t s) {
-    if (nb == 1) launch_qt<1, BITS, T>(a, qt, blocks, s);
-    else if (nb == 2) launch_qt<2, BITS, T>(a, qt, blocks, s);
-    else if (nb == 3) launch_qt<3, BITS, T>(a, qt, blocks, s);
-    else launch_qt<4, BITS, T>(a, qt, blocks, s);
+template <int NB, int BITS, typename T>
+int launch_qt(const AttnCacheArgs& a, int qt, unsigned blocks, hipStream_t s) {
+    if (a.wide) return qt == 1 ? launch_wide<NB, BITS, T, 1>(a, blocks, s) : launch_wide<NB, BITS, T, 2>(a, blocks, s);
+    if (qt == 1) hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 1>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
+    return OTTER_OK;
+}
+
+template <typename T, int BITS> int launch_nb(const AttnCacheArgs& a, int nb, int qt, unsigned blocks, hipStream_t s) {
+    if (nb == 1) return launch_qt<1, BITS, T>(a, qt, blocks, s);
+    if (nb == 2) return launch_qt<2, BITS, T>(a, qt, blocks, s);
+    if (nb == 3) return launch_qt<3, BITS, T>(a, qt, blocks, s);
+    return launch_qt<4, BITS, T>(a, qt, blocks, s);
 }
 
 }  // namespace
 
 template <typename T> int otter_attn_cache_launch(const AttnCacheArgs& a, int nb, int bits, int qt, unsigned blocks, hipStream_t s) {
-    if (bits == 4) launch_nb<T, 4>(a, nb, qt, blocks, s);
-    else launch_nb<T, 8>(a, nb, qt, blocks, s);
+    if (int rc = bits == 4 ? launch_nb<T, 4>(a, nb, qt, blocks, s) : launch_nb<T, 8>(a, nb, qt, blocks, s)) return rc;
     OTTER_CHECK_LAUNCH("otter_attn_cache");
     if (a.nsplit > 1) {
-        const dim3 grid((unsigned)(a.g.n * a.g.H * a.N));           // (bounded with the launch's own grid: columns <= 32 per group and item)
-        if (nb == 1) hipLaunchKernelGGL((attn_cache_join_kernel<T, 1>), grid, dim3(256), 0, s, a, 16 * qt);
-        else if (nb == 2) hipLaunchKernelGGL((attn_cache_join_kernel<T, 2>), grid, dim3(256), 0, s, a, 16 * qt);
-        else if (nb == 3) hipLaunchKernelGGL((attn_cache_join_kernel<T, 3>), grid, dim3(256), 0, s, a, 16 * qt);
-        else hipLaunchKernelGGL((attn_cache_join_kernel<T, 4>), grid, dim3(256), 0, s, a, 16 * qt);
+        const dim3 grid((unsigned)(a.g.n * a.g.H * a.N));           // (splits are made for at most 4096 items of at most 128 columns)
+        const int cols = (a.wide ? 64 : 16) * qt;
+        if (nb == 1) hipLaunchKernelGGL((attn_cache_join_kernel<T, 1>), grid, dim3(256), 0, s, a, cols);
+        else if (nb == 2) hipLaunchKernelGGL((attn_cache_join_kernel<T, 2>), grid, dim3(256), 0, s, a, cols);
+        else if (nb == 3) hipLaunchKernelGGL((attn_cache_join_kernel<T, 3>), grid, dim3(256), 0, s, a, cols);
+        else hipLaunchKernelGGL((attn_cache_join_kernel<T, 4>), grid, dim3(256), 0, s, a, cols);
         OTTER_CHECK_LAUNCH("otter_attn_cache (join)");
     }
     return OTTER_OK;

@@ -245,13 +245,22 @@ def test_attend_split_keys(dev, dtype, bits, d, heads, kv_heads, t):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("t,heads", [(1, 2), (40, 2), (3, 4)])
+@pytest.mark.parametrize("bits,d,heads,kv_heads,t,capacity,kw", [
+    (4, 64, 2, 2, 130, 1500, {}), (8, 96, 4, 2, 101, 1300, {"window": 333}), (4, 128, 3, 1, 67, 2100, {}), (8, 32, 2, 1, 200, 900, {"max_len": 800}),
+    (4, 96, 2, 2, 140, 700, {"causal": False})])
+def test_attend_chunk_after_a_long_history(dev, dtype, bits, d, heads, kv_heads, t, capacity, kw):
+    """Many columns, few rows: workgroups that convert the tiles together, and several of them share the keys."""
+    _check(dev, 26, bits, dtype, d, 2, t, heads, kv_heads, capacity, [capacity - t, capacity // 3], **kw)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,heads", [(1, 2), (40, 2), (3, 4), (100, 4)])
 def test_not_a_number_in_masked_places(dev, dtype, t, heads):
     """Rows that a query must not see hold NaN (and codes and scales that the writer never makes): before its window, behind its
     position, behind the length, in other episodes.  Where it does see one, its output is NaN as the formula's is."""
     from otter_amd import ops
-    bits, d, h, s, n = 4, 64, 2, 120, 3
-    pos, window = [10, 40, 70], 25
+    bits, d, h, s, n = 4, 64, 2, 220, 3
+    pos, window = [10, 40, 110], 25
     codes, scales, k, v = _filled(dev, 21, n, h, s, d, bits)
     q = _randn(22, n, t, heads, d).to(dtype)
     want = ops.attn_cache(q.to(dev), codes, scales, _i32(pos, dev), window=window)
