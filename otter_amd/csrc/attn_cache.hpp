@@ -266,16 +266,19 @@ __device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2 * NS], WaveS
             const float m4 = fmaxf(fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])), fmaxf(fmaxf(x[u][4], x[u][5]), fmaxf(x[u][6], x[u][7])));
             mx = u ? fmaxf(mx, m4) : m4;
         }
+        // The state moves to a new reference only when a score passes the old one by more than 2^8 (weights then stay below 2^8:
+        // no precision is lost, fp32 and bf16 have the range): with the running maximum itself some column of 16 moves in most
+        // tiles, and every move costs a multiplication per accumulator.
         mx = rows_max(mx);
-        const float mn = fmaxf(st.m[t], mx);
-        const float mc = mn == -INFINITY ? 0.f : mn * c;
-        if (__any(mn > st.m[t])) {
-            const float corr = __builtin_amdgcn_exp2f(st.m[t] * c - mc);
+        if (__any(__builtin_fmaf(mx, c, -st.m[t] * c) > 8.f || st.m[t] == -INFINITY)) {
+            const float mn = fmaxf(st.m[t], mx);
+            const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m[t] - mn) * c);
+            st.m[t] = mn;
             st.l[t] *= corr;
 #pragma unroll
             for (int j = 0; j < DV; ++j) st.acc[t][j] *= corr;
         }
-        st.m[t] = mn;
+        const float mc = st.m[t] == -INFINITY ? 0.f : st.m[t] * c;
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
             float p[8];
@@ -309,9 +312,9 @@ __device__ __forceinline__ void tile_values(const RawTile<NB, BITS>& r, WaveStat
             vf[1][i >> 1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
         }
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
+        for (int n = NP - 1; n >= 0; --n)
 #pragma unroll
-            for (int n = NP - 1; n >= 0; --n)
+            for (int t = 0; t < QT; ++t)
 #pragma unroll
                 for (int o = 0; o < 2; ++o)
                     st.acc[t][2 * j + o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[o]), pf[t][n], st.acc[t][2 * j + o], 0, 0, 0);
@@ -782,18 +785,20 @@ __global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a
         if (work) {
             f32x4 s[QT][4];
 #pragma unroll
-            for (int hh = 0; hh < 4; ++hh) {
+            for (int hh = 0; hh < 4; ++hh)
 #pragma unroll
                 for (int t = 0; t < QT; ++t) s[t][hh] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            // (neighbouring products go to different accumulators: one that waits for its predecessor stalls the matrix pipe)
 #pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    const bf16x8 kf = *(const bf16x8*)(buf + (hh * NB + j) * 1024 + lane * 16);
+            for (int n = NQ - 1; n >= 0; --n)
 #pragma unroll
-                    for (int t = 0; t < QT; ++t)
+                for (int j = 0; j < NB; ++j)
 #pragma unroll
-                        for (int n = NQ - 1; n >= 0; --n) s[t][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][n][j], s[t][hh], 0, 0, 0);
-                }
-            }
+                    for (int hh = 0; hh < 4; ++hh) {
+                        const bf16x8 kf = *(const bf16x8*)(buf + (hh * NB + j) * 1024 + lane * 16);
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) s[t][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][n][j], s[t][hh], 0, 0, 0);
+                    }
             const bool masked = k0 + 63 > own.hi_all || k0 + 64 > stop || k0 < own.lo_all;
             tile_weights<NB, BITS, T, QT, 2>(s, st, pf, k0, masked, lo, hi, a.c, lane);
         }
@@ -805,12 +810,14 @@ __global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int j = 0; j < DV; ++j) {
-                    const bf16x8 vf = *(const bf16x8*)(buf + (4 * NB + x * DV + j) * 1024 + lane * 16);
+                for (int j = 0; j < DV; j += 2) {
+                    const bf16x8 vf[2] = {*(const bf16x8*)(buf + (4 * NB + x * DV + j) * 1024 + lane * 16), *(const bf16x8*)(buf + (4 * NB + x * DV + j + 1) * 1024 + lane * 16)};
 #pragma unroll
-                    for (int t = 0; t < QT; ++t)
+                    for (int n = NP - 1; n >= 0; --n)
 #pragma unroll
-                        for (int n = NP - 1; n >= 0; --n) st.acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[x][t][n], st.acc[t][j], 0, 0, 0);
+                        for (int t = 0; t < QT; ++t)
+#pragma unroll
+                            for (int o = 0; o < 2; ++o) st.acc[t][j + o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[o], pf[x][t][n], st.acc[t][j + o], 0, 0, 0);
                 }
             if (edge(k0)) {
 #pragma unroll
