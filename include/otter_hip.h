@@ -369,7 +369,7 @@ int otter_kv_cache_read(const otter_kv_cache* cache, const otter_kv_rows* rows, 
  * k_new / v_new (both or none; steps == 1, count NULL): the step's own key and value, quantised, stored at pos[e] and attended to by the
  * same launch -- as otter_kv_cache_write followed by this call.
  * workspace: otter_attn_cache_workspace_floats(...) floats, 8-byte aligned, private to the call until it has run (0: none). */
-long otter_attn_cache_workspace_floats(int n_rows, int steps, int q_heads, int kv_heads, int head_dim, int window, int max_len);
+long otter_attn_cache_workspace_floats(int dtype, int n_rows, int steps, int q_heads, int kv_heads, int head_dim, int window, int max_len);
 int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* q, int q_heads,
                      const otter_kv_operand* k_new, const otter_kv_operand* v_new, const otter_kv_operand* out, int causal,
                      int window, int max_len, float scale, float* workspace, long workspace_floats, void* stream);

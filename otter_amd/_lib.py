@@ -141,7 +141,7 @@ def load() -> ctypes.CDLL:
     lib.otter_gemm_static_ws_init.restype = c_int
     lib.otter_gemm_static_ws_init.argtypes = []
     lib.otter_attn_cache_workspace_floats.restype = c_long
-    lib.otter_attn_cache_workspace_floats.argtypes = [c_int] * 7
+    lib.otter_attn_cache_workspace_floats.argtypes = [c_int] * 8
     _lib = lib
     return lib
 

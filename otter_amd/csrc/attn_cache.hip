@@ -13,11 +13,12 @@ inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 // converted tiles.
 // Keys: one wave (wide: one workgroup) walks over all of them while there are enough to fill the chip, four waves and several
 // workgroups share them otherwise.
-Plan plan(int n, int H, int steps, int G, int window, int max_len) {
+Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max_len) {
     Plan p{};
     const long U = (long)n * H, N = (long)steps * G;
     p.wide = N > 32 && steps > 1;
-    p.qt = N <= 16 || (p.wide && N <= 64) ? 1 : 2;
+    // (wide with 96 or 128 numbers a head and more than one term a query: 32 columns a wave do not fit the registers)
+    p.qt = N <= 16 || (p.wide && (N <= 64 || (nb >= 3 && dtype != DT_BF16))) ? 1 : 2;
     const long cols = (p.wide ? 64L : 16L) * p.qt;
     p.cg = (int)ceil_div(N, cols);
     const long span = (window > 0 ? std::min<long>(max_len, (long)window + cols / G + 1) : max_len) + 31;   // keys one item may walk over
@@ -39,10 +40,10 @@ Plan plan(int n, int H, int steps, int G, int window, int max_len) {
 
 }  // namespace
 
-extern "C" long otter_attn_cache_workspace_floats(int n_rows, int steps, int q_heads, int kv_heads, int head_dim, int window, int max_len) {
+extern "C" long otter_attn_cache_workspace_floats(int dtype, int n_rows, int steps, int q_heads, int kv_heads, int head_dim, int window, int max_len) {
     if (n_rows <= 0 || steps <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0 || head_dim <= 0 || max_len <= 0 || window < 0) return 0;
     if ((long)steps * (q_heads / kv_heads) >= (1L << 31) || (long)n_rows * kv_heads >= (1L << 31)) return 0;
-    const Plan p = plan(n_rows, kv_heads, steps, q_heads / kv_heads, window, max_len);
+    const Plan p = plan(dtype, head_dim / 32, n_rows, kv_heads, steps, q_heads / kv_heads, window, max_len);
     return p.nsplit > 1 ? (long)p.nsplit * n_rows * q_heads * steps * (head_dim + 2) : 0;
 }
 
@@ -70,7 +71,7 @@ extern "C" int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows
     const int G = q_heads / cache->heads;
     OTTER_REQUIRE((long)rows->steps * G < (1L << 30) && (long)rows->n_rows * cache->heads < (1L << 30), OTTER_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, heads or steps", name);
     const int cap = std::min(max_len, cache->capacity);
-    Plan p = plan(rows->n_rows, cache->heads, rows->steps, G, window, cap);
+    Plan p = plan(dtype, cache->head_dim / 32, rows->n_rows, cache->heads, rows->steps, G, window, cap);
     OTTER_REQUIRE(p.ok, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: grid too large", name);
     if (p.nsplit > 1) {
         const long need = (long)p.nsplit * rows->n_rows * q_heads * rows->steps * (cache->head_dim + 2);

@@ -81,7 +81,7 @@ __device__ __forceinline__ int v_row(int g, int i) { return 4 * g + (i & 3) + 16
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const unsigned char* base, int k0, int row_bytes, int rows) {
     const unsigned long long at = (unsigned long long)base + (unsigned long long)k0 * row_bytes;
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)at), hi = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(min(rows, 32) * row_bytes), 0x00027000);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(min(max(rows, 0), 32) * row_bytes), 0x00027000);   // no rows: everything reads as zeros
 }
 template <int BYTES, int W> __device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, unsigned (&w)[W]) {
     if constexpr (BYTES == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b8(r, off, 0, 0);

@@ -745,7 +745,7 @@ def _attn_cache(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], codes, scal
         return out
     if c.episodes == 0:
         raise ValueError(f"{name}: the cache has no episodes")
-    need = _lib.load().otter_attn_cache_workspace_floats(n, steps, hq, c.heads, d, window, cap)
+    need = _lib.load().otter_attn_cache_workspace_floats(dt, n, steps, hq, c.heads, d, window, cap)
     # the call's own scratch, from the allocator of the stream (or the graph being captured) it runs on
     ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
     _kv_call(dev, "otter_attn_cache", c, r, dt, qo, hq, ko, vo, _lib.KvOperand(out.data_ptr(), steps * hq * d, hq * d, d), int(bool(causal)),
