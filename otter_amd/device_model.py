@@ -26,6 +26,7 @@ import torch
 
 from .torch_ops import kernels as ops      # every kernel launch below is a torch.ops.otter_hip.* call
 from .config import ClipArch
+from .kv_cache import KVCache
 from .pooling import PoolingWeights
 
 Tensor = torch.Tensor
@@ -255,45 +256,74 @@ class PolicyDevice:
         self.w_h2, self.b_h2 = ops.pack_weight(sd["action_head.mlp.2.weight"].float(), torch.float32, device), _f32(sd["action_head.mlp.2.bias"], device)
         self.n_out = sd["action_head.mlp.2.weight"].shape[0]
 
-    def new_cache(self, batch: int, window: int) -> List[Tensor]:
-        """Per-layer fp32 q|k|v rows (B, window, 3*dim): the GPU-resident K/V history."""
-        return [torch.zeros(batch, window, 3 * self.dim, dtype=torch.float32, device=self.device) for _ in self.layers]
+    def new_cache(self, batch: int, window: int, kv_bits: Optional[int] = None) -> list:
+        """Per-layer GPU-resident K/V history: fp32 q|k|v rows (B, window, 3*dim), or with ``kv_bits`` 4 / 8 quantised keys and
+        values (:class:`otter_amd.kv_cache.KVCache`, no limit on the window)."""
+        if kv_bits is None:
+            return [torch.zeros(batch, window, 3 * self.dim, dtype=torch.float32, device=self.device) for _ in self.layers]
+        return [KVCache(batch, self.heads, window, self.dim // self.heads, kv_bits, self.device) for _ in self.layers]
 
-    def run(self, window: Tensor, cache: List[Tensor], n_query: int, pos0: int) -> Tensor:
+    def _qkv(self, rows: Tensor, *lead: int):
+        """q, k, v views (*lead, heads, head_dim) of fp32 q|k|v rows."""
+        t = rows.view(*lead, 3, self.heads, self.dim // self.heads)
+        return t.select(-3, 0), t.select(-3, 1), t.select(-3, 2)
+
+    def _positions(self, batch: int, window: int) -> Tensor:
+        """(window, B) int32, row p = position p for every episode."""
+        key = (batch, window)
+        if getattr(self, "_pos_key", None) != key:
+            self._pos_key = key
+            self._pos = torch.arange(window, dtype=torch.int32, device=self.device)[:, None].expand(window, batch).contiguous()
+        return self._pos
+
+    def run(self, window: Tensor, cache: list, n_query: int, pos0: int, idx: Optional[Tensor] = None) -> Tensor:
         """Run positions pos0 .. pos0+n_query-1 of every episode; returns the fp32 outputs (B*n_query, dim).
 
         ``window`` (B, S, dim) holds the policy inputs; K/V of the processed positions are written into ``cache``
-        and earlier positions are read from it.
+        and earlier positions are read from it.  ``idx`` (int32, whole windows into a quantised cache only): row i of ``window``
+        is episode ``idx[i]`` of the cache.
         """
         b, s, _ = window.shape
+        if n_query != s and n_query != 1:
+            raise ValueError("policy.run: n_query must be 1 (cached step) or the whole window")
+        if idx is not None and (n_query != s or not isinstance(cache[0], KVCache)):
+            raise ValueError("policy.run: idx goes with whole windows and a quantised cache")
         x = ops.add_pe(window, self.pe, n_query, pos0)
         f32 = torch.float32
         for blk, kv in zip(self.layers, cache):
             h = ops.layernorm(x, *blk.ln1, out_dtype=f32)
-            if n_query == s:
-                out = kv.view(b * s, 3 * self.dim)
-            elif n_query == 1:
-                out = kv[:, pos0, :]                                   # rows strided by S*3*dim
+            if isinstance(kv, KVCache):
+                fresh = ops.gemm(h, blk.wqkv, blk.n_qkv, blk.bqkv)
+                if n_query == s:
+                    q, k, v = self._qkv(fresh, b, s)
+                    kv.write(k, v, idx=idx)
+                    a = kv.attend(q, idx=idx, max_len=s).view(b * s, self.dim)
+                else:
+                    a = kv.step(*self._qkv(fresh, b), self._positions(b, s)[pos0], max_len=pos0 + 1).view(b, self.dim)
             else:
-                raise ValueError("policy.run: n_query must be 1 (cached step) or the whole window")
-            ops.gemm(h, blk.wqkv, blk.n_qkv, blk.bqkv, out=out)
-            a = ops.attn_policy(kv, n_query, pos0, self.heads)
+                out = kv.view(b * s, 3 * self.dim) if n_query == s else kv[:, pos0, :]      # (one position: rows strided by S*3*dim)
+                ops.gemm(h, blk.wqkv, blk.n_qkv, blk.bqkv, out=out)
+                a = ops.attn_policy(kv, n_query, pos0, self.heads)
             ops.gemm(a, blk.wo, blk.width, blk.bo, residual=x, out=x)
             h = ops.layernorm(x, *blk.ln2, out_dtype=f32)
             m = ops.gemm(h, blk.w_fc, blk.n_fc, blk.b_fc, act=ops.ACT_GELU)
             ops.gemm(m, blk.w_proj, blk.width, blk.b_proj, residual=x, out=x)
         return x
 
-    def run_rows(self, window: Tensor, cache: List[Tensor], idx: Tensor, lens: Tensor) -> Tensor:
+    def run_rows(self, window: Tensor, cache: list, idx: Tensor, lens: Tensor, max_len: Optional[int] = None) -> Tensor:
         """The newest position of the episodes listed in ``idx`` (int32, device), each at its own window position
-        ``lens[e] - 1`` (``lens``: int32 (B,), lengths after this step's append): only those rows are computed, their K/V are
-        stored into ``cache`` and earlier positions are read from it.  Returns fp32 (len(idx), dim)."""
+        ``lens[e] - 1`` (``lens``: int32 (B,), lengths after this step's append; none is above ``max_len``): only those rows are
+        computed, their K/V are stored into ``cache`` and earlier positions are read from it.  Returns fp32 (len(idx), dim)."""
         x = ops.add_pe_rows(window, self.pe, idx, lens)
         f32 = torch.float32
+        pos = lens - 1 if isinstance(cache[0], KVCache) else None
         for blk, kv in zip(self.layers, cache):
             h = ops.layernorm(x, *blk.ln1, out_dtype=f32)
             fresh = ops.gemm(h, blk.wqkv, blk.n_qkv, blk.bqkv)
-            a = ops.attn_policy_rows(fresh, kv, idx, lens, self.heads)
+            if pos is not None:
+                a = kv.step(*self._qkv(fresh, x.shape[0]), pos, idx, max_len=max_len).view(-1, self.dim)
+            else:
+                a = ops.attn_policy_rows(fresh, kv, idx, lens, self.heads)
             ops.gemm(a, blk.wo, blk.width, blk.bo, residual=x, out=x)
             h = ops.layernorm(x, *blk.ln2, out_dtype=f32)
             m = ops.gemm(h, blk.w_fc, blk.n_fc, blk.b_fc, act=ops.ACT_GELU)

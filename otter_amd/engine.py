@@ -82,16 +82,19 @@ class BatchedRollout:
 
     A step in which every episode is cached at one common position, or every episode recomputes, runs over the whole
     batch with no gather; a mixed step runs the two groups one after the other on their own rows.  ``reset(ids)`` of a
-    subset therefore never takes the K/V cache away from the other episodes."""
+    subset therefore never takes the K/V cache away from the other episodes.
 
-    def __init__(self, dev: OtterDevice, n_episodes: int):
-        self.dev, self.n = dev, int(n_episodes)
+    ``kv_bits`` = 4 or 8 keeps the history quantised (:class:`otter_amd.kv_cache.KVCache`): an eighth (a quarter) of the
+    memory, and windows of more than 64 positions; the actions then carry the format's rounding."""
+
+    def __init__(self, dev: OtterDevice, n_episodes: int, kv_bits: Optional[int] = None):
+        self.dev, self.n, self.kv_bits = dev, int(n_episodes), kv_bits
         self.S = dev.seq_length
         d = dev.device
         self._win = [torch.zeros(self.n, self.S, dev.dim, dtype=torch.float32, device=d) for _ in range(2)]
         self._lens = [torch.zeros(self.n, dtype=torch.int32, device=d) for _ in range(2)]
         self._cur = 0
-        self._cache = dev.policy.new_cache(self.n, self.S)
+        self._cache = dev.policy.new_cache(self.n, self.S, kv_bits)
         self.lens_host = np.zeros(self.n, dtype=np.int64)
         self.kv_ok = np.ones(self.n, dtype=bool)       # K/V rows [0, len) of the episode are valid at their current positions
         self._graph: Optional[_EncodeGraph] = None
@@ -193,11 +196,15 @@ class BatchedRollout:
             self.last_mode = "mixed" if ids_f.size else "cached"
             out = torch.empty(self.n, dev.horizon * dev.action_dim, dtype=torch.float32, device=dev.device)
             i32, i64 = self._index(ids_c)
-            out.index_copy_(0, i64, pol.head(pol.run_rows(win, self._cache, i32, lens)))
+            out.index_copy_(0, i64, pol.head(pol.run_rows(win, self._cache, i32, lens, int(self.lens_host[ids_c].max()))))
             if ids_f.size:
                 i32, i64 = self._index(ids_f)
                 win_f = win.index_select(0, i64)
                 lens_f = lens.index_select(0, i64)
-                y = pol.run(win_f, pol.new_cache(ids_f.size, self.S), self.S, 0)     # a scratch cache: these rows are not kept
+                if self.kv_bits is None:
+                    y = pol.run(win_f, pol.new_cache(ids_f.size, self.S), self.S, 0)     # a scratch cache: these rows are not kept
+                else:
+                    y = pol.run(win_f, self._cache, self.S, 0, i32)                      # into the episodes' own rows
+                    self.kv_ok[ids_f] |= before[ids_f] < self.S
                 out.index_copy_(0, i64, pol.head(y, pick=lens_f, group=self.S, pick_bias=-1))
         return out.view(self.n, dev.horizon, dev.action_dim)

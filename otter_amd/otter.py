@@ -70,6 +70,9 @@ class OTTER(nn.Module):
         # Operand type of the text tower: None = fp16 whatever the vision tower uses (bf16 rounding of the text tower alone
         # costs more action error than the tolerance allows; the tower runs once per prompt and is 0.8 % of the work).
         self.clip_text_dtype = None
+        # K/V history of forward_inference: None = fp32 rows (windows of at most 64 steps); 4 or 8 = quantised
+        # (otter_amd.kv_cache.KVCache).  Takes effect with the next rollout state (a new model, moved or reloaded weights).
+        self.kv_cache_bits: Optional[int] = None
         self._dev: Optional[OtterDevice] = None
         self._dev_key = None
         self._clip_dev: Optional[ClipDevice] = None
@@ -187,7 +190,7 @@ class OTTER(nn.Module):
     def _get_rollout(self) -> BatchedRollout:
         dev = self.device_model()
         if self._rollout is None:
-            self._rollout = BatchedRollout(dev, 1)
+            self._rollout = BatchedRollout(dev, 1, self.kv_cache_bits)
             self.cache_size = 0
             carried, self._carry_window = self._carry_window, None
             if carried is not None:

@@ -94,13 +94,15 @@ class BatchedRolloutPolicy:
     ``OTTER.forward_inference`` does), and when that changed -- an optimizer step, ``load_state_dict``,
     ``invalidate_device_weights()`` -- the running episodes' windows move over to the new weights."""
 
-    def __init__(self, model, n_episodes: int, action_exec_horizon: int, receding_horizon_control: bool = False):
+    def __init__(self, model, n_episodes: int, action_exec_horizon: int, receding_horizon_control: bool = False,
+                 kv_bits: Optional[int] = None):
+        """``kv_bits`` (4 or 8): the episodes' K/V history is kept quantised (:class:`otter_amd.engine.BatchedRollout`)."""
         from .engine import BatchedRollout
         if action_exec_horizon > model.action_horizon:
             raise ValueError(f"action_exec_horizon must be at most the predicted horizon ({model.action_horizon})")
         self.model = model
         self.dev = model.device_model()
-        self.rollout = BatchedRollout(self.dev, n_episodes)
+        self.rollout = BatchedRollout(self.dev, n_episodes, kv_bits)
         self.queue = DeviceActionQueue(n_episodes, action_exec_horizon, self.dev.device, receding_horizon_control, action_dim=model.action_dim)
         self.n = int(n_episodes)
 
@@ -113,7 +115,7 @@ class BatchedRolloutPolicy:
         from .engine import BatchedRollout
         dev = self.model.device_model()
         if dev is not self.dev:
-            fresh = BatchedRollout(dev, self.n)
+            fresh = BatchedRollout(dev, self.n, self.rollout.kv_bits)
             fresh.adopt(self.rollout)              # policy inputs of the running episodes are kept, K/V rows are recomputed
             self.dev, self.rollout = dev, fresh
 
