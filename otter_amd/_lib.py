@@ -153,6 +153,22 @@ def call(name: str, *args) -> None:
         raise OtterHipError(f"{name} failed (code {rc}): {lib.otter_last_error().decode()}")
 
 
+_packed: dict = {}
+
+
+def call_packed(name: str, *args) -> None:
+    """:func:`call` for entry points that take struct pointers, with the structs as packed bytes."""
+    fn = _packed.get(name)
+    if fn is None:
+        fn = load()[name]                # a function object of its own: the one in ``load()`` keeps its struct argument types
+        fn.argtypes = [c_void_p if a in (_KC, _KR, _KO) else a for a in _SIGNATURES[name]]
+        fn.restype = c_int
+        _packed[name] = fn
+    rc = fn(*args)
+    if rc != 0:
+        raise OtterHipError(f"{name} failed (code {rc}): {load().otter_last_error().decode()}")
+
+
 def exported_names():
     return sorted(list(_SIGNATURES) + ["otter_last_error", "otter_hip_abi_version", "otter_grad_stats_workspace_floats",
                                             "otter_pos_emb_packed_elems", "otter_gemm_workspace_floats", "otter_gemm_static_ws_max_n",

@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 import threading
 from typing import Optional, Sequence
 
@@ -36,7 +37,8 @@ def _dt(dtype, name: str, allow_f32: bool = True) -> int:
 
 
 def _stream() -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # (the raw handle: building torch's Stream object costs more host time than a small kernel takes)
+    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _chk(t: Tensor, dtype, name: str, dims: Optional[int] = None) -> Tensor:
@@ -623,61 +625,74 @@ def action_step(delta_chunks: Tensor, cur_pose: Tensor, ring: Tensor, counts: Te
 
 
 # ------------------------------------------------------------------------------------------------------ quantised K/V cache
-def _kv_operand(t: Tensor, dtype, shape: tuple, name: str, device) -> "_lib.KvOperand":
+# A serving step makes one or two of these calls per layer on sizes whose kernels take a few microseconds, so the path from the
+# tensors to the call is kept short: the C structs are packed in one step each (layouts of _lib.KvCache, KvRows, KvOperand).
+_PACK_CACHE, _PACK_ROWS, _PACK_OPERAND = struct.Struct("@PlllPllliiiii4x").pack, struct.Struct("@PPPii").pack, struct.Struct("@Plll").pack
+
+
+def _kv_operand(t: Tensor, dtype, shape: tuple, name: str, device) -> bytes:
     """A (row, step, head, dim) tensor with free strides outside the last dimension."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or tuple(t.shape) != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != device:
         _chk(t, dtype, name)
         raise ValueError(f"{name}: {tuple(t.shape)} on {t.device}, expected {shape} on {device}")
     sr, ss, sh, sd = t.stride()
     if sd != 1:
         raise ValueError(f"{name}: innermost dimension must be contiguous")
-    n, steps, h, _ = shape
-    return _lib.KvOperand(t.data_ptr(), sr if n > 1 else 0, ss if steps > 1 else 0, sh if h > 1 else 0)
+    return _PACK_OPERAND(t.data_ptr(), sr if shape[0] > 1 else 0, ss if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
 
 
-def _kv_cache(codes: Tensor, scales: Tensor, head_dim: int, name: str) -> "_lib.KvCache":
-    _chk(codes, torch.uint8, name + ".codes", 5)
-    _chk(scales, torch.uint8, name + ".scales", 5)
+def _kv_cache(codes: Tensor, scales: Tensor, head_dim: int, name: str):
+    """-> (packed otter_kv_cache, episodes, heads, capacity)."""
+    if not isinstance(codes, torch.Tensor) or codes.dtype != torch.uint8 or codes.dim() != 5 or not codes.is_cuda:
+        _chk(codes, torch.uint8, name + ".codes", 5)
+    if not isinstance(scales, torch.Tensor) or scales.dtype != torch.uint8 or scales.dim() != 5 or not scales.is_cuda:
+        _chk(scales, torch.uint8, name + ".scales", 5)
     two, e, h, s, row = codes.shape
-    bits = {head_dim // 2: 4, head_dim: 8}.get(row)
-    if two != 2 or tuple(scales.shape) != (2, e, h, s, 4) or bits is None or scales.device != codes.device:
+    bits = 4 if row * 2 == head_dim else 8
+    if two != 2 or scales.shape != (2, e, h, s, 4) or (bits == 8 and row != head_dim) or scales.device != codes.device:
         raise ValueError(f"{name}: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} for head_dim {head_dim}: "
                          "(2, episodes, heads, capacity, head_dim / 2 or head_dim) and (2, episodes, heads, capacity, 4)")
-    if head_dim % 32 != 0 or not 32 <= head_dim <= 128:
+    if head_dim not in (32, 64, 96, 128):
         raise ValueError(f"{name}: head_dim {head_dim} must be 32, 64, 96 or 128")
     if s == 0 or h == 0:
         raise ValueError(f"{name}: the cache holds no positions or no heads")
-    cs, ss = codes.stride(), scales.stride()
-    if (s > 1 and (cs[3] != row or ss[3] != 4)) or cs[4] != 1 or ss[4] != 1:
+    ckv, ce, ch, cs, c1 = codes.stride()
+    skv, se, sh, ss, s1 = scales.stride()
+    if (s > 1 and (cs != row or ss != 4)) or c1 != 1 or s1 != 1:
         raise ValueError(f"{name}: the positions of a head must be contiguous")
-    return _lib.KvCache(codes.data_ptr(), cs[0], cs[1] if e > 1 else 0, cs[2] if h > 1 else 0,
-                        scales.data_ptr(), ss[0], ss[1] if e > 1 else 0, ss[2] if h > 1 else 0, bits, e, h, s, head_dim)
+    if e <= 1:
+        ce = se = 0
+    if h == 1:
+        ch = sh = 0
+    return _PACK_CACHE(codes.data_ptr(), ckv, ce, ch, scales.data_ptr(), skv, se, sh, bits, e, h, s, head_dim), e, h, s
 
 
-def _kv_index(t: Optional[Tensor], length: int, name: str, device) -> Optional[int]:
+def _kv_index(t: Optional[Tensor], length: int, name: str, device) -> int:
     if t is None:
-        return None
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != device or t.dim() != 1 or t.shape[0] != length or not t.is_contiguous():
+        return 0
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (length,) or t.device != device or not t.is_contiguous():
         _chk(t, torch.int32, name, 1)
         raise ValueError(f"{name}: {tuple(t.shape)} on {t.device}, expected a contiguous ({length},) on {device}")
     return t.data_ptr()
 
 
-def _kv_rows(cache: "_lib.KvCache", device, n: int, steps: int, pos: Optional[Tensor], idx: Optional[Tensor], count: Optional[Tensor],
-             name: str) -> "_lib.KvRows":
-    if idx is None and n > cache.episodes:
-        raise ValueError(f"{name}: {n} rows without idx, cache of {cache.episodes} episodes")
-    return _lib.KvRows(_kv_index(idx, n, name + ".idx", device), _kv_index(pos, cache.episodes, name + ".pos", device),
-                       _kv_index(count, n, name + ".count", device), n, steps)
+def _kv_rows(episodes: int, device, n: int, steps: int, pos: Optional[Tensor], idx: Optional[Tensor], count: Optional[Tensor], name: str) -> bytes:
+    if idx is None and n > episodes:
+        raise ValueError(f"{name}: {n} rows without idx, cache of {episodes} episodes")
+    if not (0 <= n < 1 << 31 and 0 <= steps <= 1 << 30):
+        raise ValueError(f"{name}: {n} rows of {steps} steps")
+    return _PACK_ROWS(_kv_index(idx, n, name + ".idx", device), _kv_index(pos, episodes, name + ".pos", device),
+                      _kv_index(count, n, name + ".count", device), n, steps)
 
 
 def _kv_call(device, fn: str, *args) -> None:
     """Launch on the cache's device, on that device's current stream."""
-    if device.index == torch.cuda.current_device():
-        _lib.call(fn, *args, _stream())
+    index = device.index
+    if index == torch.cuda.current_device():
+        _lib.call_packed(fn, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            _lib.call(fn, *args, _stream())
+            _lib.call_packed(fn, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def kv_cache_write(k: Tensor, v: Tensor, codes: Tensor, scales: Tensor, pos: Optional[Tensor] = None, idx: Optional[Tensor] = None,
@@ -691,12 +706,12 @@ def kv_cache_write(k: Tensor, v: Tensor, codes: Tensor, scales: Tensor, pos: Opt
         raise ValueError("kv_cache_write: k must be (n, steps, heads, head_dim)")
     n, steps, h, d = k.shape
     dt = _dt(k.dtype, "kv_cache_write.k")
-    c = _kv_cache(codes, scales, d, "kv_cache_write")
+    c, episodes, heads, _ = _kv_cache(codes, scales, d, "kv_cache_write")
     dev = codes.device
-    if h != c.heads:
-        raise ValueError(f"kv_cache_write: {h} heads, cache of {c.heads}")
+    if h != heads:
+        raise ValueError(f"kv_cache_write: {h} heads, cache of {heads}")
     ko, vo = _kv_operand(k, k.dtype, (n, steps, h, d), "kv_cache_write.k", dev), _kv_operand(v, k.dtype, (n, steps, h, d), "kv_cache_write.v", dev)
-    r = _kv_rows(c, dev, n, steps, pos, idx, count, "kv_cache_write")
+    r = _kv_rows(episodes, dev, n, steps, pos, idx, count, "kv_cache_write")
     if n and steps:
         _kv_call(dev, "otter_kv_cache_write", c, r, dt, ko, vo)
 
@@ -707,17 +722,15 @@ def kv_cache_read(codes: Tensor, scales: Tensor, head_dim: int, steps: int, pos:
     in ``dtype``; rows as in :func:`kv_cache_write` (without ``idx``: the first ``n_rows`` episodes, all by default).  What the
     cache does not hold, and steps at or past count[i], read as zeros."""
     dt = _dt(dtype, "kv_cache_read.dtype")
-    c = _kv_cache(codes, scales, head_dim, "kv_cache_read")
+    c, episodes, h, _ = _kv_cache(codes, scales, head_dim, "kv_cache_read")
     dev = codes.device
-    if steps < 0:
-        raise ValueError("kv_cache_read: negative steps")
-    n = idx.shape[0] if idx is not None else c.episodes if n_rows is None else int(n_rows)
-    r = _kv_rows(c, dev, n, int(steps), pos, idx, count, "kv_cache_read")
-    k = torch.empty(n, steps, c.heads, head_dim, dtype=dtype, device=dev)
+    n = idx.shape[0] if idx is not None else episodes if n_rows is None else int(n_rows)
+    r = _kv_rows(episodes, dev, n, int(steps), pos, idx, count, "kv_cache_read")
+    k = torch.empty((n, steps, h, head_dim), dtype=dtype, device=dev)
     v = torch.empty_like(k)
     if n and steps:
-        sr, ss, sh, _ = k.stride()
-        _kv_call(dev, "otter_kv_cache_read", c, r, dt, _lib.KvOperand(k.data_ptr(), sr, ss, sh), _lib.KvOperand(v.data_ptr(), sr, ss, sh))
+        sh, ss = head_dim, h * head_dim
+        _kv_call(dev, "otter_kv_cache_read", c, r, dt, _PACK_OPERAND(k.data_ptr(), steps * ss, ss, sh), _PACK_OPERAND(v.data_ptr(), steps * ss, ss, sh))
     return k, v
 
 
@@ -725,30 +738,32 @@ def _attn_cache(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], codes, scal
                 scale: Optional[float], max_len: Optional[int], name: str) -> Tensor:
     n, steps, hq, d = q.shape
     dt = _dt(q.dtype, name + ".q")
-    c = _kv_cache(codes, scales, d, name)
+    c, episodes, h, cap = _kv_cache(codes, scales, d, name)
     dev = codes.device
-    if hq == 0 or hq % c.heads != 0:
-        raise ValueError(f"{name}: {hq} query heads over {c.heads} key heads")
+    if hq == 0 or hq % h != 0:
+        raise ValueError(f"{name}: {hq} query heads over {h} key heads")
     if window < 0 or (max_len is not None and max_len < 1):
         raise ValueError(f"{name}: window={window}, max_len={max_len}")
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 3.0e38:
         raise ValueError(f"{name}: scale must be positive and finite")
-    cap = c.capacity if max_len is None else min(int(max_len), c.capacity)
+    if max_len is not None and max_len < cap:
+        cap = int(max_len)
+    window = min(window, 1 << 30)
     qo = _kv_operand(q, q.dtype, (n, steps, hq, d), name + ".q", dev)
     ko = vo = None
     if k is not None:
-        ko, vo = _kv_operand(k, q.dtype, (n, 1, c.heads, d), name + ".k", dev), _kv_operand(v, q.dtype, (n, 1, c.heads, d), name + ".v", dev)
-    r = _kv_rows(c, dev, n, steps, pos, idx, count, name)
-    out = torch.empty(n, steps, hq, d, dtype=q.dtype, device=dev)
+        ko, vo = _kv_operand(k, q.dtype, (n, 1, h, d), name + ".k", dev), _kv_operand(v, q.dtype, (n, 1, h, d), name + ".v", dev)
+    r = _kv_rows(episodes, dev, n, steps, pos, idx, count, name)
+    out = torch.empty((n, steps, hq, d), dtype=q.dtype, device=dev)
     if n == 0 or steps == 0:
         return out
-    if c.episodes == 0:
+    if episodes == 0:
         raise ValueError(f"{name}: the cache has no episodes")
-    need = _lib.load().otter_attn_cache_workspace_floats(dt, n, steps, hq, c.heads, d, window, cap)
+    need = _lib.load().otter_attn_cache_workspace_floats(dt, n, steps, hq, h, d, window, cap)
     # the call's own scratch, from the allocator of the stream (or the graph being captured) it runs on
-    ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
-    _kv_call(dev, "otter_attn_cache", c, r, dt, qo, hq, ko, vo, _lib.KvOperand(out.data_ptr(), steps * hq * d, hq * d, d), int(bool(causal)),
+    ws = torch.empty((need,), dtype=torch.float32, device=dev) if need else None
+    _kv_call(dev, "otter_attn_cache", c, r, dt, qo, hq, ko, vo, _PACK_OPERAND(out.data_ptr(), steps * hq * d, hq * d, d), 1 if causal else 0,
              window, cap, scale, None if ws is None else ws.data_ptr(), need)
     return out
 
