@@ -498,6 +498,22 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
     int lo[QT], hi[QT], col[QT];
     lane_columns<QT>(a, r, c0, li, col, lo, hi);
 
+    TileSource src;
+    {
+        const long e = max(r.e, 0);
+        src.k = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
+        src.v = src.k + a.g.ckv;
+        src.ks = a.g.scales + e * a.g.se + (long)h * a.g.sh;
+        src.vs = src.ks + a.g.skv;
+    }
+    WaveState<NB, BITS, T, QT> st;
+    const int first = start + (a.kw == 4 ? 32 * w : 0), stride = a.kw * 32;
+    // one tile's registers: the next keys are requested once the scores stand, the next values once the second product has read its own
+    RawTile<NB, BITS> raw;
+    if (first < stop) {                                            // on their way while the fresh row and the queries are dealt with
+        load_keys<NB, BITS>(raw, src, first, stop - first, lane);
+        load_values<NB, BITS>(raw, src, first, stop - first, lane);
+    }
     // the fresh row: codes to the cache and, for this wave's own tiles, to LDS
     unsigned char* fr = fresh_rows[w];
     int fresh_pos = -1;
@@ -508,7 +524,13 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
         int from = i;                                              // an episode listed twice: the last listing is the one that is stored and seen
         if (a.g.idx) {
             int last = i;
-            for (int j = i + 1 + lane; j < a.g.n; j += 64) last = a.g.idx[j] == r.e ? j : last;
+            for (int j0 = i + 1; j0 < a.g.n; j0 += 512) {          // eight loads in flight
+                int other[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) { const int j = j0 + 64 * q + lane; other[q] = j < a.g.n ? a.g.idx[j] : -1; }
+#pragma unroll
+                for (int q = 0; q < 8; ++q) last = other[q] == r.e ? j0 + 64 * q + lane : last;
+            }
 #pragma unroll
             for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
             from = __builtin_amdgcn_readfirstlane(last);
@@ -543,19 +565,6 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
 
     bf16x8 qf[QT][NQ][NB];
     load_queries<NB, T, QT>(a, i, h, col, g, qf);
-
-    TileSource src;
-    {
-        const long e = max(r.e, 0);
-        src.k = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
-        src.v = src.k + a.g.ckv;
-        src.ks = a.g.scales + e * a.g.se + (long)h * a.g.sh;
-        src.vs = src.ks + a.g.skv;
-    }
-    WaveState<NB, BITS, T, QT> st;
-    const int first = start + (a.kw == 4 ? 32 * w : 0), stride = a.kw * 32;
-    // one tile's registers: the next keys are requested once the scores stand, the next values once the second product has read its own
-    RawTile<NB, BITS> raw;
     auto keys = [&](int k0) {
         load_keys<NB, BITS>(raw, src, k0, stop - k0, lane);
         if (fresh_pos >= k0 && fresh_pos < k0 + 32) take_fresh_key<NB, BITS>(raw, fr, k0, fresh_pos, lane);
@@ -566,9 +575,9 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
     };
     st.reset();
     float mark[QT] = {};
-    if (first < stop) {
-        keys(first);
-        values(first);
+    if (fresh_pos >= first && fresh_pos < first + 32) {
+        take_fresh_key<NB, BITS>(raw, fr, first, fresh_pos, lane);
+        take_fresh_value<NB, BITS>(raw, fr, first, fresh_pos, lane);
     }
     for (int k0 = first; k0 < stop; k0 += stride) {
         const bool more = k0 + stride < stop;
@@ -843,16 +852,18 @@ __global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a
     store_columns<NB, BITS, T, QT>(a, st, u, i, h, sp, col, lo, hi, g);
 }
 
-// The splits of one column put together.  A workgroup takes one column; D / 4 lanes read one split's numbers, so 8 to 32 splits
-// are in flight at a time (read one after the other by one wave, 32 splits cost 15 us of memory round trips, now 4.x).
-template <typename T, int NB>
+// The splits of one column put together.  WV waves take one column; D / 4 lanes read one split's numbers, so several splits are in
+// flight at a time (read one after the other by one wave, 32 splits cost 15 us of memory round trips; four waves: 4 us).
+template <typename T, int NB, int WV>
 __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, int cols_per_group) {
-    constexpr int D = 32 * NB, LPS = D / 4, PAR = 256 / LPS;       // lanes per split, splits at a time
-    __shared__ float red[4];
-    __shared__ __attribute__((aligned(16))) f32x4 sums[PAR][LPS];
-    __shared__ float ls[PAR];
+    constexpr int D = 32 * NB, LPS = D / 4, PAR = 64 * WV / LPS, CPB = 4 / WV;       // lanes per split, splits at a time, columns a workgroup
+    __shared__ __attribute__((aligned(16))) f32x4 sums[CPB][PAR][LPS];
+    __shared__ float red[4], ls[CPB][PAR];
     const int U = a.g.n * a.g.H;
-    const int u = blockIdx.x / a.N, c = blockIdx.x - u * a.N;
+    const int tid = threadIdx.x % (64 * WV), cw = threadIdx.x / (64 * WV);
+    const int item = blockIdx.x * CPB + cw;
+    const bool live = item < U * a.N;
+    const int u = live ? item / a.N : 0, c = live ? item - u * a.N : 0;
     const int i = u / a.g.H, h = u - i * a.g.H, step = c / a.G, hq = h * a.G + c - step * a.G;
     const KvRow r = kv_row(a.g, i);
     const int c0 = c / cols_per_group * cols_per_group;
@@ -861,16 +872,19 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, i
     const int ns = max((kr.end - (kr.beg & ~31) + a.chunk - 1) / a.chunk, 1);       // splits that this column's group really has
     const long hop = (long)U * a.N * (D + 2);
     const float* base = a.part + ((long)u * a.N + c) * (D + 2);
-    const int tid = threadIdx.x, q = tid % LPS, w = tid / LPS;
+    const int q = tid % LPS, w = tid / LPS;
     float m = -INFINITY;
-    for (int s = tid; s < ns; s += 256) m = fmaxf(m, base[s * hop + D]);
+    for (int s = tid; s < ns; s += 64 * WV) m = fmaxf(m, base[s * hop + D]);
     m = wave_max(m);
-    if ((tid & 63) == 0) red[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if constexpr (WV > 1) {
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
     float l = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    if (w < PAR)
+    if (w < PAR) {
+#pragma unroll 4
         for (int s = w; s < ns; s += PAR) {
             const float* y = base + s * hop;
             const f32x2 v0 = *(const f32x2*)(y + 4 * q), v1 = *(const f32x2*)(y + 4 * q + 2), ml = *(const f32x2*)(y + D);
@@ -878,18 +892,17 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, i
             l += ml[1] * f;
             o += (f32x4){v0[0], v0[1], v1[0], v1[1]} * f;
         }
-    if (w < PAR) {
-        sums[w][q] = o;
-        if (q == 0) ls[w] = l;
+        sums[cw][w][q] = o;
+        if (q == 0) ls[cw][w] = l;
     }
     __syncthreads();
-    if (tid >= LPS) return;
+    if (tid >= LPS || !live) return;
     const int parts = min(PAR, ns);
-    o = sums[0][tid];
-    l = ls[0];
+    o = sums[cw][0][tid];
+    l = ls[cw][0];
     for (int k = 1; k < parts; ++k) {                              // fixed order
-        o += sums[k][tid];
-        l += ls[k];
+        o += sums[cw][k][tid];
+        l += ls[cw][k];
     }
     const bool none = own.beg >= own.end;
     const float inv = 1.0f / l;
@@ -902,6 +915,12 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, i
         for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.f : o[e] * inv);
         *(typename Half16<T>::v4*)y = v;
     }
+}
+
+template <typename T, int NB> void launch_join(const AttnCacheArgs& a, int cols, hipStream_t s) {
+    const unsigned items = (unsigned)(a.g.n * a.g.H * a.N);         // (splits are made for at most 4096 items of at most 128 columns)
+    if (a.nsplit <= 8) hipLaunchKernelGGL((attn_cache_join_kernel<T, NB, 1>), dim3((items + 3) / 4), dim3(256), 0, s, a, cols);
+    else hipLaunchKernelGGL((attn_cache_join_kernel<T, NB, 4>), dim3(items), dim3(256), 0, s, a, cols);
 }
 
 template <int NB, int BITS, typename T, int QT>
@@ -933,12 +952,11 @@ template <typename T> int otter_attn_cache_launch(const AttnCacheArgs& a, int nb
     if (int rc = bits == 4 ? launch_nb<T, 4>(a, nb, qt, blocks, s) : launch_nb<T, 8>(a, nb, qt, blocks, s)) return rc;
     OTTER_CHECK_LAUNCH("otter_attn_cache");
     if (a.nsplit > 1) {
-        const dim3 grid((unsigned)(a.g.n * a.g.H * a.N));           // (splits are made for at most 4096 items of at most 128 columns)
         const int cols = (a.wide ? 64 : 16) * qt;
-        if (nb == 1) hipLaunchKernelGGL((attn_cache_join_kernel<T, 1>), grid, dim3(256), 0, s, a, cols);
-        else if (nb == 2) hipLaunchKernelGGL((attn_cache_join_kernel<T, 2>), grid, dim3(256), 0, s, a, cols);
-        else if (nb == 3) hipLaunchKernelGGL((attn_cache_join_kernel<T, 3>), grid, dim3(256), 0, s, a, cols);
-        else hipLaunchKernelGGL((attn_cache_join_kernel<T, 4>), grid, dim3(256), 0, s, a, cols);
+        if (nb == 1) launch_join<T, 1>(a, cols, s);
+        else if (nb == 2) launch_join<T, 2>(a, cols, s);
+        else if (nb == 3) launch_join<T, 3>(a, cols, s);
+        else launch_join<T, 4>(a, cols, s);
         OTTER_CHECK_LAUNCH("otter_attn_cache (join)");
     }
     return OTTER_OK;

@@ -631,14 +631,15 @@ _PACK_CACHE, _PACK_ROWS, _PACK_OPERAND = struct.Struct("@PlllPllliiiii4x").pack,
 
 
 def _kv_operand(t: Tensor, dtype, shape: tuple, name: str, device) -> bytes:
-    """A (row, step, head, dim) tensor with free strides outside the last dimension."""
+    """A (row, step, head, dim) or (row, head, dim) tensor with free strides outside the last dimension."""
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape or t.device != device:
         _chk(t, dtype, name)
         raise ValueError(f"{name}: {tuple(t.shape)} on {t.device}, expected {shape} on {device}")
-    sr, ss, sh, sd = t.stride()
-    if sd != 1:
+    strides = t.stride()
+    if strides[-1] != 1:
         raise ValueError(f"{name}: innermost dimension must be contiguous")
-    return _PACK_OPERAND(t.data_ptr(), sr if shape[0] > 1 else 0, ss if shape[1] > 1 else 0, sh if shape[2] > 1 else 0)
+    return _PACK_OPERAND(t.data_ptr(), strides[0] if shape[0] > 1 else 0, strides[1] if len(shape) == 4 and shape[1] > 1 else 0,
+                         strides[-2] if shape[-2] > 1 else 0)
 
 
 def _kv_cache(codes: Tensor, scales: Tensor, head_dim: int, name: str):
@@ -736,7 +737,9 @@ def kv_cache_read(codes: Tensor, scales: Tensor, head_dim: int, steps: int, pos:
 
 def _attn_cache(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], codes, scales, pos, idx, count, causal: bool, window: int,
                 scale: Optional[float], max_len: Optional[int], name: str) -> Tensor:
-    n, steps, hq, d = q.shape
+    shape = q.shape
+    n, hq, d = shape[0], shape[-2], shape[-1]
+    steps = shape[1] if len(shape) == 4 else 1
     dt = _dt(q.dtype, name + ".q")
     c, episodes, h, cap = _kv_cache(codes, scales, d, name)
     dev = codes.device
@@ -750,12 +753,12 @@ def _attn_cache(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], codes, scal
     if max_len is not None and max_len < cap:
         cap = int(max_len)
     window = min(window, 1 << 30)
-    qo = _kv_operand(q, q.dtype, (n, steps, hq, d), name + ".q", dev)
+    qo = _kv_operand(q, q.dtype, shape, name + ".q", dev)
     ko = vo = None
     if k is not None:
-        ko, vo = _kv_operand(k, q.dtype, (n, 1, h, d), name + ".k", dev), _kv_operand(v, q.dtype, (n, 1, h, d), name + ".v", dev)
+        ko, vo = _kv_operand(k, q.dtype, (n, h, d), name + ".k", dev), _kv_operand(v, q.dtype, (n, h, d), name + ".v", dev)
     r = _kv_rows(episodes, dev, n, steps, pos, idx, count, name)
-    out = torch.empty((n, steps, hq, d), dtype=q.dtype, device=dev)
+    out = torch.empty(shape, dtype=q.dtype, device=dev)
     if n == 0 or steps == 0:
         return out
     if episodes == 0:
@@ -788,8 +791,7 @@ def attn_cache_rows(q: Tensor, k: Tensor, v: Tensor, codes: Tensor, scales: Tens
     for t, nm in ((q, "q"), (k, "k"), (v, "v")):
         if not isinstance(t, torch.Tensor) or t.dim() != 3:
             raise ValueError(f"attn_cache_rows: {nm} must be (n, heads, head_dim)")
-    return _attn_cache(q.unsqueeze(1), k.unsqueeze(1), v.unsqueeze(1), codes, scales, pos, idx, None, True, int(window), scale, max_len,
-                       "attn_cache_rows").squeeze(1)
+    return _attn_cache(q, k, v, codes, scales, pos, idx, None, True, int(window), scale, max_len, "attn_cache_rows")
 
 
 # ------------------------------------------------------------------------------------------------------ training step
