@@ -5,17 +5,18 @@
 
 namespace {
 
-struct Plan { int qt, wide, cg, kw, nsplit, chunk; unsigned blocks; bool ok; };
+struct Plan { int qt, vec, wide, cg, kw, nsplit, chunk; unsigned blocks; bool ok; };
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-// Columns: 16 per wave while all of a row's columns fit, then 32; from 33 on, with several steps, four waves share the
+// One step with one or two query heads a key head: the vector form.  Columns otherwise: 16 per wave while all of a row's columns fit, then 32; from 33 on, with several steps, four waves share the
 // converted tiles.
 // Keys: one wave (wide: one workgroup) walks over all of them while there are enough to fill the chip, four waves and several
 // workgroups share them otherwise.
 Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max_len) {
     Plan p{};
     const long U = (long)n * H, N = (long)steps * G;
+    p.vec = steps == 1 && G <= 2;
     p.wide = N > 32 && steps > 1;
     // (wide with 96 or 128 numbers a head and more than one term a query: 32 columns a wave do not fit the registers)
     // (and 32 only where that leaves two waves a SIMD: few waves are a matter of latency, not of conversions)
@@ -96,6 +97,7 @@ extern "C" int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows
     a.window = window;
     a.max_len = cap;
     a.c = scale * 1.44269504088896341f;
+    a.vec = p.vec;
     a.wide = p.wide;
     a.kw = p.kw;
     a.nsplit = p.nsplit;

@@ -28,6 +28,7 @@ struct AttnCacheArgs {
     int G, N, CG;                                   // query heads per key head, columns T * G, column groups of 16 * QT (64 * QT: wide)
     int causal, window, max_len;
     float c;
+    int vec;                                        // 1: one step, one or two columns, on the vector unit
     int wide;                                       // 1: four waves x 16 QT columns a workgroup over tiles that they convert together
     int kw, nsplit, chunk;                          // waves per item along the keys (1 or 4), splits of the key range, keys per split (multiple of 32 * kw)
     float* part;                                    // [nsplit][n * H][N][D + 2] partial sums: D numbers, maximum, sum
@@ -78,10 +79,10 @@ __device__ __forceinline__ int v_row(int g, int i) { return 4 * g + (i & 3) + 16
 // Rows are read through buffer resources that end with the tile's last existing row: what lies behind reads as zeros (checked
 // word by word; scale byte 0 with codes 0 is the number 0), so a ragged tile needs no addresses of its own, and every load is a
 // 32-bit lane offset from a scalar base.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const unsigned char* base, int k0, int row_bytes, int rows) {
+template <int MOST = 32> __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(const unsigned char* base, int k0, int row_bytes, int rows) {
     const unsigned long long at = (unsigned long long)base + (unsigned long long)k0 * row_bytes;
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)at), hi = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(min(max(rows, 0), 32) * row_bytes), 0x00027000);   // no rows: everything reads as zeros
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(min(max(rows, 0), MOST) * row_bytes), 0x00027000);   // no rows: everything reads as zeros
 }
 template <int BYTES, int W> __device__ __forceinline__ void buffer_words(__amdgpu_buffer_rsrc_t r, int off, unsigned (&w)[W]) {
     if constexpr (BYTES == 1) w[0] = __builtin_amdgcn_raw_buffer_load_b8(r, off, 0, 0);
@@ -358,12 +359,15 @@ template <int NB, int BITS>
 __device__ __forceinline__ void take_fresh_key(RawTile<NB, BITS>& r, const unsigned char* fresh, int k0, int pos, int lane) {
     constexpr int RB = 4 * NB * BITS, KB = RB / 4, KW = RawTile<NB, BITS>::KW;
     const int li = lane & 15, g = lane >> 4;
+    unsigned kw[KW];                                               // (read by all lanes, then selected: a read under the condition is a branch a word)
+    lds_words<KB>(fresh + g * KB, kw);
+    const unsigned ks = *(const unsigned*)(fresh + 2 * RB);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const bool here = k0 + li + 16 * h == pos;
 #pragma unroll
-        for (int i = 0; i < KW; ++i) r.k[h][i] = here ? *(const unsigned*)(fresh + g * KB + 4 * i) : r.k[h][i];
-        r.ks[h] = here ? *(const unsigned*)(fresh + 2 * RB) : r.ks[h];
+        for (int i = 0; i < KW; ++i) r.k[h][i] = here ? kw[i] : r.k[h][i];
+        r.ks[h] = here ? ks : r.ks[h];
     }
 }
 template <int NB, int BITS>
@@ -457,6 +461,62 @@ __device__ __forceinline__ void store_columns(const AttnCacheArgs& a, const Wave
     }
 }
 
+// The step's own key and value (args.kn, args.vn): codes to the cache (`stores`: one wave of the item) and to this wave's LDS
+// row `fr` -- codes of the key, of the value, then their scale words -- for the tile that holds its position.  Returns that
+// position if it lies in [start, stop), -1 otherwise.
+template <int NB, int BITS, typename T>
+__device__ __forceinline__ int append_row(const AttnCacheArgs& a, const KvRow& r, int i, int h, int sp, int start, int stop, int end, bool stores,
+                                          unsigned char* fr, int lane) {
+    constexpr int RB = 4 * NB * BITS;
+    // (a position that max_len hides is stored all the same, by the first split)
+    const bool sees = r.pos >= start && r.pos < stop;
+    if (!a.kn.p || r.e < 0 || !(sees || (sp == 0 && r.pos >= end && r.pos < a.g.S))) return -1;
+    const int p = lane & 15, kv = lane >> 4;                       // lanes 0 .. 15: the key row, 16 .. 31: the value row, 8 numbers each
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const bool on = lane < 32 && p < 4 * NB;
+    const KvOperand<const void>& o = kv ? a.vn : a.kn;
+    if (on) kv_load8<T>((const T*)o.p + (long)i * o.row + (long)h * o.head + 8 * p, a.new_vec, x);
+    int from = i;                                                  // an episode listed twice: the last listing is the one that is stored and seen
+    if (a.g.idx) {
+        int last = i;
+        for (int j0 = i + 1; j0 < a.g.n; j0 += 512) {              // eight loads in flight
+            int other[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) other[q] = a.g.idx[min(j0 + 64 * q + lane, a.g.n - 1)];
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                const int j = j0 + 64 * q + lane;
+                last = j < a.g.n && other[q] == r.e ? j : last;
+            }
+        }
+        if (__any(last != i)) {
+#pragma unroll
+            for (int q = 32; q > 0; q >>= 1) last = max(last, __shfl_xor(last, q, 64));
+            from = __builtin_amdgcn_readfirstlane(last);
+            if (on) kv_load8<T>((const T*)o.p + (long)from * o.row + (long)h * o.head + 8 * p, a.new_vec, x);
+        }
+    }
+    const unsigned sb = kv_scale_byte<BITS>(kv_block_top(x));
+    unsigned cw[BITS / 4];
+    kv_encode8<BITS>(x, sb, cw);
+    if (lane < 2) *(unsigned*)(fr + 2 * RB + 4 * lane) = 0u;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (on) {
+#pragma unroll
+        for (int q = 0; q < BITS / 4; ++q) *(unsigned*)(fr + kv * RB + p * BITS + 4 * q) = cw[q];
+        if ((p & 3) == 0) fr[2 * RB + 4 * kv + (p >> 2)] = (unsigned char)sb;
+        if (from == i && stores) {
+            unsigned char* cc = a.g.codes + kv * a.g.ckv + (long)r.e * a.g.ce + (long)h * a.g.ch + (long)r.pos * RB + p * BITS;
+            if constexpr (BITS == 4) *(unsigned*)cc = cw[0];
+            else *(uint2*)cc = make_uint2(cw[0], cw[BITS / 4 - 1]);
+            if ((p & 3) == 0) a.g.scales[kv * a.g.skv + (long)r.e * a.g.se + (long)h * a.g.sh + (long)r.pos * 4 + (p >> 2)] = (unsigned char)sb;
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return sees ? r.pos : -1;
+}
+
 // Items: (split, row, key head, column group).  A workgroup of four waves takes one item with the keys dealt out in tiles
 // (kw = 4), or four items: neighbouring column groups of one (row, head), which read the same rows, or, with one column
 // group, four (row, head) pairs.  (row, head) runs fastest over the workgroups, so that the column groups of one pair meet in
@@ -514,55 +574,8 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
         load_keys<NB, BITS>(raw, src, first, stop - first, lane);
         load_values<NB, BITS>(raw, src, first, stop - first, lane);
     }
-    // the fresh row: codes to the cache and, for this wave's own tiles, to LDS
     unsigned char* fr = fresh_rows[w];
-    int fresh_pos = -1;
-    // (a position that max_len hides is stored all the same, by the first split)
-    const bool sees_fresh = r.pos >= start && r.pos < stop;
-    if (a.kn.p && r.e >= 0 && (sees_fresh || (sp == 0 && r.pos >= kr.end && r.pos < a.g.S))) {
-        fresh_pos = sees_fresh ? r.pos : -1;
-        int from = i;                                              // an episode listed twice: the last listing is the one that is stored and seen
-        if (a.g.idx) {
-            int last = i;
-            for (int j0 = i + 1; j0 < a.g.n; j0 += 512) {          // eight loads in flight
-                int other[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) { const int j = j0 + 64 * q + lane; other[q] = j < a.g.n ? a.g.idx[j] : -1; }
-#pragma unroll
-                for (int q = 0; q < 8; ++q) last = other[q] == r.e ? j0 + 64 * q + lane : last;
-            }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) last = max(last, __shfl_xor(last, o, 64));
-            from = __builtin_amdgcn_readfirstlane(last);
-        }
-        const int kv = lane >> 4, p = li;                          // lanes 0 .. 15: the key row, 16 .. 31: the value row, 8 numbers each
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const bool on = lane < 32 && p < 4 * NB;
-        if (on) {
-            const KvOperand<const void>& o = kv ? a.vn : a.kn;
-            kv_load8<T>((const T*)o.p + (long)from * o.row + (long)h * o.head + 8 * p, a.new_vec, x);
-        }
-        const unsigned sb = kv_scale_byte<BITS>(kv_block_top(x));
-        unsigned cw[BITS / 4];
-        kv_encode8<BITS>(x, sb, cw);
-        if (lane < 2) *(unsigned*)(fr + 2 * RB + 4 * lane) = 0u;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (on) {
-#pragma unroll
-            for (int q = 0; q < BITS / 4; ++q) *(unsigned*)(fr + kv * RB + p * BITS + 4 * q) = cw[q];
-            if ((p & 3) == 0) fr[2 * RB + 4 * kv + (p >> 2)] = (unsigned char)sb;
-            // one wave of the item writes the row: the first of the group with key 0's columns
-            if (from == i && cg == 0 && (a.kw == 1 || w == 0)) {
-                unsigned char* cc = a.g.codes + kv * a.g.ckv + (long)r.e * a.g.ce + (long)h * a.g.ch + (long)r.pos * RB + p * BITS;
-                if constexpr (BITS == 4) *(unsigned*)cc = cw[0];
-                else *(uint2*)cc = make_uint2(cw[0], cw[BITS / 4 - 1]);
-                if ((p & 3) == 0) a.g.scales[kv * a.g.skv + (long)r.e * a.g.se + (long)h * a.g.sh + (long)r.pos * 4 + (p >> 2)] = (unsigned char)sb;
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    }
-
+    const int fresh_pos = append_row<NB, BITS, T>(a, r, i, h, sp, start, stop, kr.end, cg == 0 && (a.kw == 1 || w == 0), fr, lane);
     bf16x8 qf[QT][NQ][NB];
     load_queries<NB, T, QT>(a, i, h, col, g, qf);
     auto keys = [&](int k0) {
@@ -852,6 +865,291 @@ __global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a
     store_columns<NB, BITS, T, QT>(a, st, u, i, h, sp, col, lo, hi, g);
 }
 
+// ------------------------------------------------------------------------------------------------
+// One new position and one or two query heads per key head (NC columns): a matrix instruction would use 1 or 2 of its 16 columns
+// and the wave would still pay for the terms and the transposition, so this form stays on the vector unit in fp32: a tile is 64
+// keys, one a lane for the scores (the query's numbers come from LDS, the same address for all lanes), and one row of 16 lanes
+// per 16 keys for the sum of the values (lane = 8 numbers, the weight of key i broadcast within the row by DPP).  About 360
+// vector instructions per 64 keys at head_dim 96 against 1100 issue slots of the matrix form in fp32, and registers for four waves a
+// SIMD: all 4096 waves of a 512-episode step are resident at once.  Measured against the matrix form (us, graph replay): 512 rows x
+// 8 heads x 96, 32 positions, fp32 9.1 : 11.2; 64 x 8 x 128, 4096 positions, 4 bits, fp32 60 : 104, bf16 59 : 71, 8 bits 110 : 108
+// (memory); two heads a key head, 64 x 16 / 8 x 128, 4096 positions, bf16 70 : 68, fp16 in 8 bits 105 : 123.
+template <int NB, int BITS> struct VecTile {
+    static constexpr int KW = 4 * NB * BITS / 4;                   // words of a whole row
+    static constexpr int DV = RawTile<NB, BITS>::DV, VW = RawTile<NB, BITS>::VW;
+    unsigned k[KW], ks, v[16][VW], vs[16];
+};
+template <int NB, int BITS> __device__ __forceinline__ void vec_load(VecTile<NB, BITS>& r, const TileSource& src, int k0, int rows, int lane) {
+    constexpr int RB = 4 * NB * BITS, VB = VecTile<NB, BITS>::DV * BITS / 8;
+    const int li = lane & 15, g = lane >> 4;
+    const auto kc = rows_of<64>(src.k, k0, RB, rows), ks = rows_of<64>(src.ks, k0, 4, rows);
+    buffer_words<RB>(kc, lane * RB, r.k);
+    r.ks = __builtin_amdgcn_raw_buffer_load_b32(ks, lane * 4, 0, 0);
+    const auto vc = rows_of<64>(src.v, k0, RB, rows), vs = rows_of<64>(src.vs, k0, 4, rows);
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const auto u = __builtin_amdgcn_raw_buffer_load_b128(vs, 64 * g + 4 * i, 0, 0);
+        r.vs[i] = u[0]; r.vs[i + 1] = u[1]; r.vs[i + 2] = u[2]; r.vs[i + 3] = u[3];
+    }
+    const int vl = (NB == 3 ? min(li, 11) : li) * VB + 16 * g * RB;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) buffer_words<VB>(vc, vl + i * RB, r.v[i]);
+}
+
+// two numbers (word w, pair j of it) as floats
+template <int BITS> __device__ __forceinline__ f32x2 decode2(unsigned w, int j, float sc) {
+    if constexpr (BITS == 4) {
+        if (j == 0) return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 0);
+        if (j == 1) return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 1);
+        if (j == 2) return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 2);
+        return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, sc, 3);
+    } else {
+        if (j == 0) return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, sc, false);
+        return __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w, sc, true);
+    }
+}
+
+// value of lane I of the row of 16 lanes, in every lane of the row
+template <int I> __device__ __forceinline__ float row_lane(float v) { return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x150 + I, 0xF, 0xF, true)); }
+
+template <int NB, int BITS, int NC, int I = 0>
+__device__ __forceinline__ void vec_values(const VecTile<NB, BITS>& r, const float (&p)[NC], float (&acc)[NC][RawTile<NB, BITS>::DV], int block) {
+    if constexpr (I < 16) {
+        constexpr int DV = RawTile<NB, BITS>::DV, PPW = 16 / BITS;  // pairs a word
+        const float sc = scale_of(r.vs[I], block);
+        float w[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) w[c] = row_lane<I>(p[c]);
+#pragma unroll
+        for (int j = 0; j < DV / 2; ++j) {
+            const f32x2 y = decode2<BITS>(r.v[I][j / PPW], j % PPW, sc);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                acc[c][2 * j] = __builtin_fmaf(w[c], y[0], acc[c][2 * j]);
+                acc[c][2 * j + 1] = __builtin_fmaf(w[c], y[1], acc[c][2 * j + 1]);
+            }
+        }
+        if constexpr (I % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        vec_values<NB, BITS, NC, I + 1>(r, p, acc, block);
+    }
+}
+
+// maximum / sum over the wave, vector instructions only: within a row of 16 by DPP, then over the four rows
+__device__ __forceinline__ float dpp_xor1(float v) { return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0xB1, 0xF, 0xF, true)); }
+__device__ __forceinline__ float dpp_xor2(float v) { return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x4E, 0xF, 0xF, true)); }
+__device__ __forceinline__ float dpp_half_mirror(float v) { return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x141, 0xF, 0xF, true)); }
+__device__ __forceinline__ float dpp_mirror(float v) { return __uint_as_float((unsigned)__builtin_amdgcn_mov_dpp((int)__float_as_uint(v), 0x140, 0xF, 0xF, true)); }
+__device__ __forceinline__ float all_max(float v) {
+    v = fmaxf(v, dpp_xor1(v));
+    v = fmaxf(v, dpp_xor2(v));
+    v = fmaxf(v, dpp_half_mirror(v));
+    v = fmaxf(v, dpp_mirror(v));
+    return rows_max(v);
+}
+__device__ __forceinline__ float all_sum(float v) {
+    v += dpp_xor1(v);
+    v += dpp_xor2(v);
+    v += dpp_half_mirror(v);
+    v += dpp_mirror(v);
+    return rows_sum(v);
+}
+
+template <int NB, int BITS, typename T, int NC>
+__global__ __launch_bounds__(256, (NC == 1 && (BITS == 4 || NB <= 2) ? 4 : NC == 2 && BITS == 8 && NB >= 3 ? 2 : 3)) void attn_cache_vector_kernel(AttnCacheArgs a) {
+    constexpr int D = 32 * NB, RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, KW = VecTile<NB, BITS>::KW, VW = VecTile<NB, BITS>::VW;
+    constexpr int MROW = D + 4;
+    __shared__ __attribute__((aligned(16))) unsigned char fresh_rows[4][2 * RB + 16];
+    __shared__ __attribute__((aligned(16))) float queries[4][NC][D];
+    __shared__ __attribute__((aligned(16))) float merge[4 * NC * MROW];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, g = lane >> 4;
+    const int U = a.g.n * a.g.H;
+    const int u = a.kw == 4 ? blockIdx.x % U : blockIdx.x * 4 + w, sp = a.kw == 4 ? blockIdx.x / U : 0;
+    if (u >= U) return;                                            // (only with kw = 1: no barrier follows)
+    const int i = u / a.g.H, h = u - i * a.g.H;
+    const KvRow r = kv_row(a.g, i);
+    const KeyRange kr = key_range(a, r, 0, a.N - 1);               // one step: every column sees the same keys
+    const int start = (kr.beg & ~31) + sp * a.chunk, stop = min(kr.end, start + a.chunk);
+    if (sp > 0 && start >= stop) return;                           // the whole workgroup: the item has fewer splits
+    TileSource src;
+    {
+        const long e = max(r.e, 0);
+        src.k = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
+        src.v = src.k + a.g.ckv;
+        src.ks = a.g.scales + e * a.g.se + (long)h * a.g.sh;
+        src.vs = src.ks + a.g.skv;
+    }
+    const int first = start + (a.kw == 4 ? 64 * w : 0), stride = a.kw * 64;
+    VecTile<NB, BITS> raw;
+    if (first < stop) vec_load<NB, BITS>(raw, src, first, stop - first, lane);
+
+    // queries: 8 numbers a lane to LDS
+    {
+        const int c = lane >> 4, p = li;
+        if (c < NC && p < 4 * NB) {
+            float x[8];
+            kv_load8<T>((const T*)a.q.p + (long)i * a.q.row + (long)(h * a.G + c) * a.q.head + 8 * p, a.q_vec, x);
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) *(f32x4*)(&queries[w][c][8 * p + e]) = (f32x4){x[e], x[e + 1], x[e + 2], x[e + 3]};
+        }
+    }
+    unsigned char* fr = fresh_rows[w];
+    const int fresh_pos = append_row<NB, BITS, T>(a, r, i, h, sp, start, stop, kr.end, a.kw == 1 || w == 0, fr, lane);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+
+    auto take_fresh = [&](int k0) {
+        const int at = fresh_pos - k0;
+        const unsigned ks = *(const unsigned*)(fr + 2 * RB), vs = *(const unsigned*)(fr + 2 * RB + 4);
+#pragma unroll
+        for (int q = 0; q < KW; q += 4) {                          // (read by all lanes, then selected: a read under the condition is a branch a word)
+            const u32x4 x = *(const u32x4*)(fr + 4 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw.k[q + e] = lane == at ? x[e] : raw.k[q + e];
+        }
+        raw.ks = lane == at ? ks : raw.ks;
+        constexpr int VB = DV * BITS / 8;
+        unsigned vw[VW];
+        lds_words<VB>(fr + RB + (NB == 3 ? min(li, 11) : li) * VB, vw);
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            const bool here = 16 * g + q == at;
+#pragma unroll
+            for (int x = 0; x < VW; ++x) raw.v[q][x] = here ? vw[x] : raw.v[q][x];
+            raw.vs[q] = here ? vs : raw.vs[q];
+        }
+    };
+    float m[NC], l[NC], acc[NC][DV];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        m[c] = -INFINITY;
+        l[c] = 0.f;
+#pragma unroll
+        for (int j = 0; j < DV; ++j) acc[c][j] = 0.f;
+    }
+    const int block = NB == 1 ? 0 : NB == 2 ? li >> 3 : li >> 2;
+    for (int k0 = first; k0 < stop; k0 += stride) {
+        if (fresh_pos >= k0 && fresh_pos < k0 + 64) take_fresh(k0);
+        asm volatile("" ::: "memory");                             // the queries stay in LDS: held in registers across the loop they would cost 100 of them
+        float s[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[c] = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const float sc = scale_of(raw.ks, b);
+            float part[NC][2] = {};
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {                          // four numbers at a time
+                const int word = (32 * b + 4 * q) * BITS / 32, j0 = BITS == 4 ? (q & 1) * 2 : 0;
+                const f32x2 y0 = decode2<BITS>(raw.k[word], j0, sc), y1 = decode2<BITS>(raw.k[word], j0 + 1, sc);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const f32x4 x = *(const f32x4*)&queries[w][c][32 * b + 4 * q];
+                    part[c][0] = __builtin_fmaf(y0[0], x[0], part[c][0]);
+                    part[c][1] = __builtin_fmaf(y0[1], x[1], part[c][1]);
+                    part[c][0] = __builtin_fmaf(y1[0], x[2], part[c][0]);
+                    part[c][1] = __builtin_fmaf(y1[1], x[3], part[c][1]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[c] += part[c][0] + part[c][1];
+            __builtin_amdgcn_sched_barrier(0);                     // (numbers decoded ahead of their use only fill registers)
+        }
+        const bool edge = k0 < kr.lo_all || k0 + 64 > stop;
+        if (edge) {                                                // keys behind the end, and before the window: their value rows count as zeros
+            const int key = k0 + lane;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) s[c] = key >= kr.lo_all && key < stop ? s[c] : -INFINITY;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) raw.vs[q] = k0 + 16 * g + q >= kr.lo_all ? raw.vs[q] : 0u;
+        }
+        float p[NC];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            if (__any(__builtin_fmaf(s[c], a.c, -m[c] * a.c) > 8.f) || m[c] == -INFINITY) {       // (see move_reference)
+                const float mn = fmaxf(m[c], all_max(s[c]));
+                const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[c] - mn) * a.c);
+                m[c] = mn;
+                l[c] *= corr;
+#pragma unroll
+                for (int j = 0; j < DV; ++j) acc[c][j] *= corr;
+            }
+            const float mc = m[c] == -INFINITY ? 0.f : m[c] * a.c;
+            p[c] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[c], a.c, -mc));
+            l[c] += p[c];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        vec_values<NB, BITS, NC>(raw, p, acc, block);
+        if (k0 + stride < stop) vec_load<NB, BITS>(raw, src, k0 + stride, stop - k0 - stride, lane);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        l[c] = all_sum(l[c]);
+#pragma unroll
+        for (int j = 0; j < DV; ++j) acc[c][j] = rows_sum(acc[c][j]);
+    }
+    const bool none = kr.beg >= kr.end;
+    const int lanes = D / DV;                                      // lanes of the first row that hold the numbers: DV each
+    if (a.kw == 1) {
+        if (lane < lanes)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float inv = 1.0f / l[c];
+                T* o = (T*)a.out.p + (long)i * a.out.row + (long)(h * a.G + c) * a.out.head + DV * lane;
+                typedef __attribute__((ext_vector_type(DV))) T vt;
+                vt v;
+#pragma unroll
+                for (int j = 0; j < DV; ++j) v[j] = (T)(none ? 0.f : acc[c][j] * inv);
+                if constexpr (sizeof(vt) <= 16) *(vt*)o = v;
+                else {
+                    *(f32x4*)o = (f32x4){v[0], v[1], v[2], v[3]};
+                    *(f32x4*)(o + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+                }
+            }
+        return;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        float* mine = merge + (w * NC + c) * MROW;
+        if (lane < lanes)
+#pragma unroll
+            for (int j = 0; j < DV; j += 2) *(f32x2*)(mine + DV * lane + j) = (f32x2){acc[c][j], acc[c][j + 1]};
+        if (lane == 0) { mine[D] = m[c]; mine[D + 1] = l[c]; }
+    }
+    __syncthreads();
+    for (int q = threadIdx.x; q < NC * (D / 4); q += 256) {
+        const int c = q / (D / 4), d = (q % (D / 4)) * 4;
+        float mx = -INFINITY, sum = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mx = fmaxf(mx, merge[(k * NC + c) * MROW + D]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float* from = merge + (k * NC + c) * MROW;
+            const float f = from[D] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((from[D] - mx) * a.c);
+            sum += from[D + 1] * f;
+            o += *(const f32x4*)(from + d) * f;
+        }
+        if (a.nsplit == 1) {
+            const float inv = 1.0f / sum;
+            T* y = (T*)a.out.p + (long)i * a.out.row + (long)(h * a.G + c) * a.out.head + d;
+            if constexpr (sizeof(T) == 4) {
+                *(f32x4*)y = none ? (f32x4){0.f, 0.f, 0.f, 0.f} : o * inv;
+            } else {
+                typename Half16<T>::v4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.f : o[e] * inv);
+                *(typename Half16<T>::v4*)y = v;
+            }
+        } else {
+            float* y = a.part + (((long)sp * U + u) * a.N + c) * (D + 2);
+            *(f32x2*)(y + d) = (f32x2){o[0], o[1]};
+            *(f32x2*)(y + d + 2) = (f32x2){o[2], o[3]};
+            if (d == 0) *(f32x2*)(y + D) = (f32x2){mx, sum};
+        }
+    }
+}
+
 // The splits of one column put together.  WV waves take one column; D / 4 lanes read one split's numbers, so several splits are in
 // flight at a time (read one after the other by one wave, 32 splits cost 15 us of memory round trips; four waves: 4 us).
 template <typename T, int NB, int WV>
@@ -933,6 +1231,11 @@ int launch_wide(const AttnCacheArgs& a, unsigned blocks, hipStream_t s) {
 
 template <int NB, int BITS, typename T>
 int launch_qt(const AttnCacheArgs& a, int qt, unsigned blocks, hipStream_t s) {
+    if (a.vec) {
+        if (a.G == 1) hipLaunchKernelGGL((attn_cache_vector_kernel<NB, BITS, T, 1>), dim3(blocks), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((attn_cache_vector_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
+        return OTTER_OK;
+    }
     if (a.wide) return qt == 1 ? launch_wide<NB, BITS, T, 1>(a, blocks, s) : launch_wide<NB, BITS, T, 2>(a, blocks, s);
     if (qt == 1) hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 1>), dim3(blocks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
