@@ -18,9 +18,8 @@ Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max
     const long U = (long)n * H, N = (long)steps * G;
     p.vec = steps == 1 && G <= 2;
     p.wide = N > 32 && steps > 1;
-    // (wide with 96 or 128 numbers a head and more than one term a query: 32 columns a wave do not fit the registers)
-    // (and 32 only where that leaves two waves a SIMD: few waves are a matter of latency, not of conversions)
-    p.qt = N <= 16 || (p.wide ? N <= 64 || (nb >= 3 && dtype != DT_BF16) : U * ceil_div(N, 32) < 2048) ? 1 : 2;
+    // (narrow: 32 only where that leaves two waves a SIMD: few waves are a matter of latency, not of conversions)
+    p.qt = N <= 16 || (p.wide ? N <= 64 || wide_columns(dtype, nb) == 1 : U * ceil_div(N, 32) < 2048) ? 1 : 2;
     const long cols = (p.wide ? 64L : 16L) * p.qt;
     p.cg = (int)ceil_div(N, cols);
     const long span = (window > 0 ? std::min<long>(max_len, (long)window + cols / G + 1) : max_len) + 31;   // keys one item may walk over

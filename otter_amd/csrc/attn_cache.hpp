@@ -7,6 +7,9 @@
 // v_mfma_f32_16x16x32_bf16 with fp32 accumulation.  q and p are written as sums of bf16 terms: q exactly (1 term for bf16, 2 for
 // fp16, 3 for fp32), p in 2 terms (2^-17 relative, far below the output's own rounding) for 16-bit and 3 (2^-24) for fp32 outputs.
 //
+// For 16-bit activations and many columns the second product runs on fp16 operands instead, as long as the values allow it (see
+// `Products`): fp16 weights carry 2^-12, so that bf16 outputs need one term where bf16 weights need two.
+//
 // Tile.  A wave owns 16 * QT columns (query positions x heads of one key head's group) and walks over tiles of 32 keys, all
 // state in registers.  S^T = K Q^T puts 8 scores of one column in a lane, keys 4g+i and 16+4g+i (g = lane / 16), which is the
 // B operand of out^T = V^T P^T if V's rows are taken in the same key order: no exchange between lanes.  K is loaded as it lies
@@ -54,6 +57,22 @@ template <typename T> struct AttnTerms;
 template <> struct AttnTerms<__bf16> { static constexpr int q = 1, p = 2; };
 template <> struct AttnTerms<_Float16> { static constexpr int q = 2, p = 2; };
 template <> struct AttnTerms<float> { static constexpr int q = 3, p = 3; };
+
+// Operand types and terms of the two products.  HALF: the values (and, for fp16 activations, the keys: the query is then one exact
+// term) as fp16.  A block's numbers are exact in fp16 if its exponent e leaves them between 2^-24 and 65504: -23 <= e <= 13 for
+// e2m1, -15 <= e <= 7 for e4m3 (magnitudes between about 1e-6 and 5e4); a block at the lowest exponent, -100, is zeros or below
+// 8e-30 and counts as zeros.  A workgroup that meets any other block starts over in bf16 terms.  Weights are scaled by 2^11 (below
+// 2^15 with the reference's growth of 2^4): the smallest fp16 number is then 2^-35 of the largest weight.
+template <typename T, bool HALF> struct Products { typedef __bf16 key, value; static constexpr int q = AttnTerms<T>::q, p = AttnTerms<T>::p; static constexpr float growth = 8.f, lift = 0.f; };
+template <> struct Products<__bf16, true> { typedef __bf16 key; typedef _Float16 value; static constexpr int q = 1, p = 1; static constexpr float growth = 4.f, lift = 11.f; };
+template <> struct Products<_Float16, true> { typedef _Float16 key, value; static constexpr int q = 1, p = 2; static constexpr float growth = 4.f, lift = 11.f; };
+
+// With one term a weight its sum is one more product, with a row of ones: 16 matrix cycles for 8 weights a lane where additions take 32.
+template <typename T, bool HALF> constexpr bool kSumByProduct = HALF && Products<T, HALF>::p == 1;
+
+// most columns (in units of 16) that a wave of the wide form takes: with 96 or 128 numbers a head and several terms a query, 32 do
+// not fit the registers
+constexpr int wide_columns(int dtype, int nb) { return nb <= 2 || dtype == DT_BF16 ? 2 : 1; }
 
 // host: instantiated per element type (attn_cache_*.hip)
 template <typename T> int otter_attn_cache_launch(const AttnCacheArgs& a, int nb, int bits, int qt, unsigned blocks, hipStream_t s);
@@ -143,64 +162,72 @@ __device__ __forceinline__ float scale_of(unsigned word, int block) {
     return __uint_as_float(__builtin_amdgcn_alignbit(word, word, rot));
 }
 
-// eight consecutive codes (from word w of a lane's row part on) as bf16
-template <int BITS> __device__ __forceinline__ bf16x8 decode8(const unsigned* w, float sc) {
-    bf16x2 d[4];
-    if constexpr (BITS == 4) {
-        d[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 0);
-        d[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 1);
-        d[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 2);
-        d[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 3);
-    } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            d[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[h], sc, false);
-            d[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[h], sc, true);
+// pair number j of a lane's words as two numbers of type V
+template <int BITS, typename V = __bf16> __device__ __forceinline__ unsigned decode_pair(const unsigned* w, int j, float sc) {
+    if constexpr (sizeof(V) == 2 && KvElem<V>::code == DT_F16) {
+        f16x2 d;
+        if constexpr (BITS == 4) {
+            if (j % 4 == 0) d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[j / 4], sc, 0);
+            else if (j % 4 == 1) d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[j / 4], sc, 1);
+            else if (j % 4 == 2) d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[j / 4], sc, 2);
+            else d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[j / 4], sc, 3);
+        } else {
+            if (j & 1) d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[j >> 1], sc, true);
+            else d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[j >> 1], sc, false);
         }
-    }
-    bf16x8 o;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = d[i >> 1][i & 1];
-    return o;
-}
-// pair number j of a lane's part of a value row
-template <int BITS> __device__ __forceinline__ unsigned decode_pair(const unsigned* w, int j, float sc) {
-    bf16x2 d;
-    if constexpr (BITS == 4) {
-        if (j == 0) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 0);
-        else if (j == 1) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 1);
-        else if (j == 2) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 2);
-        else d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], sc, 3);
+        return __builtin_bit_cast(unsigned, d);
     } else {
-        if (j & 1) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j >> 1], sc, true);
-        else d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j >> 1], sc, false);
+        bf16x2 d;
+        if constexpr (BITS == 4) {
+            if (j % 4 == 0) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j / 4], sc, 0);
+            else if (j % 4 == 1) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j / 4], sc, 1);
+            else if (j % 4 == 2) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j / 4], sc, 2);
+            else d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[j / 4], sc, 3);
+        } else {
+            if (j & 1) d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j >> 1], sc, true);
+            else d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j >> 1], sc, false);
+        }
+        return __builtin_bit_cast(unsigned, d);
     }
-    return __builtin_bit_cast(unsigned, d);
+}
+// eight consecutive codes (from word w of a lane's row part on)
+template <int BITS, typename V = __bf16> __device__ __forceinline__ typename Half16<V>::v8 decode8(const unsigned* w, float sc) {
+    const u32x4 d = {decode_pair<BITS, V>(w, 0, sc), decode_pair<BITS, V>(w, 1, sc), decode_pair<BITS, V>(w, 2, sc), decode_pair<BITS, V>(w, 3, sc)};
+    return __builtin_bit_cast(typename Half16<V>::v8, d);
 }
 
 __device__ __forceinline__ unsigned pack_bf16(float a, float b) {
     return __builtin_bit_cast(unsigned, (bf16x2){(__bf16)a, (__bf16)b});
 }
 
-// eight numbers as NP bf16 operands whose sum they are (to 2^-8 of the last term)
-template <int NP> __device__ __forceinline__ void split_p(const float (&p)[8], bf16x8 (&out)[NP]) {
+// eight numbers as NP operands of type V whose sum they are (to the rounding of the last term)
+template <int NP, typename V = __bf16> __device__ __forceinline__ void split_p(const float (&p)[8], typename Half16<V>::v8 (&out)[NP]) {
     unsigned w[NP][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         float a = p[2 * i], b = p[2 * i + 1];
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
-            w[n][i] = pack_bf16(a, b);
-            if (n + 1 < NP) {
-                a -= __uint_as_float(w[n][i] << 16);
-                b -= __uint_as_float(w[n][i] & 0xffff0000u);
+            if constexpr (KvElem<V>::code == DT_F16) {
+                const f16x2 h = {(_Float16)a, (_Float16)b};
+                w[n][i] = __builtin_bit_cast(unsigned, h);
+                if (n + 1 < NP) {
+                    a -= (float)h[0];
+                    b -= (float)h[1];
+                }
+            } else {
+                w[n][i] = pack_bf16(a, b);
+                if (n + 1 < NP) {
+                    a -= __uint_as_float(w[n][i] << 16);
+                    b -= __uint_as_float(w[n][i] & 0xffff0000u);
+                }
             }
         }
     }
 #pragma unroll
     for (int n = 0; n < NP; ++n) {
         const u32x4 v = {w[n][0], w[n][1], w[n][2], w[n][3]};
-        out[n] = __builtin_bit_cast(bf16x8, v);
+        out[n] = __builtin_bit_cast(typename Half16<V>::v8, v);
     }
 }
 
@@ -240,9 +267,9 @@ __device__ __forceinline__ void tile_scores(const RawTile<NB, BITS>& r, const bf
 }
 
 // scores of NS x 32 keys -> weights, as operands of the second product; the state follows the new maximum
-template <int NB, int BITS, typename T, int QT, int NS>
-__device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2 * NS], WaveState<NB, BITS, T, QT>& st, bf16x8 (&pf)[NS][QT][AttnTerms<T>::p], int k0,
-                                             bool masked, const int (&lo)[QT], const int (&hi)[QT], float c, int lane) {
+template <int NB, int BITS, typename T, int QT, int NS, bool HALF = false>
+__device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2 * NS], WaveState<NB, BITS, T, QT>& st,
+                                             typename Half16<typename Products<T, HALF>::value>::v8 (&pf)[NS][QT][Products<T, HALF>::p], f32x4 (&lsum)[QT], int k0, bool masked, const int (&lo)[QT], const int (&hi)[QT], float c, int lane) {
     constexpr int DV = RawTile<NB, BITS>::DV;
     const int g = lane >> 4;
 #pragma unroll
@@ -261,25 +288,27 @@ __device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2 * NS], WaveS
                     x[u][i] = (key <= hi[t] && key >= lo[t]) ? x[u][i] : -INFINITY;
                 }
         }
-        float mx = x[0][0];
+        // (first level by v_med3 with infinity: fmaxf would quiet every score in an instruction of its own first)
+        float mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < NS; ++u) {
-            const float m4 = fmaxf(fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])), fmaxf(fmaxf(x[u][4], x[u][5]), fmaxf(x[u][6], x[u][7])));
-            mx = u ? fmaxf(mx, m4) : m4;
-        }
-        // The state moves to a new reference only when a score passes the old one by more than 2^8 (weights then stay below 2^8:
-        // no precision is lost, fp32 and bf16 have the range): with the running maximum itself some column of 16 moves in most
+        for (int u = 0; u < NS; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                mx = fmaxf(mx, fmaxf(__builtin_amdgcn_fmed3f(x[u][i], x[u][i + 1], INFINITY), __builtin_amdgcn_fmed3f(x[u][i + 2], x[u][i + 3], INFINITY)));
+        // The state moves to a new reference only when a score passes the old one by more than 2^growth (weights then stay below
+        // 2^(growth + lift): no precision is lost, the operands have the range): with the running maximum itself some column of 16 moves in most
         // tiles, and every move costs a multiplication per accumulator.
         mx = rows_max(mx);
-        if (__any(__builtin_fmaf(mx, c, -st.m[t] * c) > 8.f || st.m[t] == -INFINITY)) {
+        if (__any(__builtin_fmaf(mx, c, -st.m[t] * c) > Products<T, HALF>::growth || st.m[t] == -INFINITY)) {
             const float mn = fmaxf(st.m[t], mx);
             const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m[t] - mn) * c);
             st.m[t] = mn;
-            st.l[t] *= corr;
+            if constexpr (kSumByProduct<T, HALF>) lsum[t] *= corr;
+            else st.l[t] *= corr;
 #pragma unroll
             for (int j = 0; j < DV; ++j) st.acc[t][j] *= corr;
         }
-        const float mc = st.m[t] == -INFINITY ? 0.f : st.m[t] * c;
+        const float mc = (st.m[t] == -INFINITY ? 0.f : st.m[t] * c) - Products<T, HALF>::lift;
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
             float p[8];
@@ -289,8 +318,8 @@ __device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2 * NS], WaveS
                 p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], c, -mc));
                 sum += p[i];
             }
-            st.l[t] += sum;
-            split_p(p, pf[u][t]);
+            if constexpr (!kSumByProduct<T, HALF>) st.l[t] += sum;
+            split_p<Products<T, HALF>::p, typename Products<T, HALF>::value>(p, pf[u][t]);
         }
     }
 }
@@ -399,9 +428,11 @@ template <int QT> __device__ __forceinline__ void lane_columns(const AttnCacheAr
 }
 
 // query operands: numbers 8 NB g + 8 j .. + 7 of the lane's column, as a sum of bf16 terms (cut, not rounded: the rest is exact)
-template <int NB, typename T, int QT>
-__device__ __forceinline__ void load_queries(const AttnCacheArgs& a, int i, int h, const int (&col)[QT], int g, bf16x8 (&qf)[QT][AttnTerms<T>::q][NB]) {
-    constexpr int NQ = AttnTerms<T>::q;
+template <int NB, typename T, int QT, bool HALF = false>
+__device__ __forceinline__ void load_queries(const AttnCacheArgs& a, int i, int h, const int (&col)[QT], int g,
+                                             typename Half16<typename Products<T, HALF>::key>::v8 (&qf)[QT][Products<T, HALF>::q][NB]) {
+    typedef typename Products<T, HALF>::key K;
+    constexpr int NQ = Products<T, HALF>::q;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         const int step = col[t] / a.G, hq = h * a.G + col[t] - step * a.G;
@@ -414,8 +445,8 @@ __device__ __forceinline__ void load_queries(const AttnCacheArgs& a, int i, int 
                 float rest = x[e];
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-                    const float cut = __uint_as_float(__float_as_uint(rest) & 0xffff0000u);
-                    qf[t][n][j][e] = (__bf16)cut;
+                    const float cut = NQ > 1 ? __uint_as_float(__float_as_uint(rest) & 0xffff0000u) : rest;
+                    qf[t][n][j][e] = (K)cut;
                     rest -= cut;
                 }
             }
@@ -599,7 +630,8 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
         bf16x8 pf[1][QT][AttnTerms<T>::p];
         tile_scores<NB, BITS, T, QT>(raw, qf, s, lane);
         if (more) keys(k0 + stride);
-        tile_weights<NB, BITS, T, QT, 1>(s, st, pf, k0, masked, lo, hi, a.c, lane);
+        f32x4 unused[QT];
+        tile_weights<NB, BITS, T, QT, 1>(s, st, pf, unused, k0, masked, lo, hi, a.c, lane);
         unsigned suspect = 0;
         if (masked) {
 #pragma unroll
@@ -710,15 +742,29 @@ template <int NB, int BITS> __device__ __forceinline__ void wide_load(WideTile<N
 }
 
 // `edge`: the tile has keys that some column does not see: blocks that are not finite are taken out and named in the masks
-template <int NB, int BITS> __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned char* buf, bool edge, int lane, int w) {
+// `least`, `most`: over the bytes met, as the top bits of a word, `least` less 28: the lowest exponent's byte 27 and the zeros of
+// rows that do not exist wrap around and pass
+template <int NB, int BITS, typename T, bool HALF>
+__device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned char* buf, bool edge, unsigned& least, unsigned& most, int lane, int w) {
     typedef WideTile<NB, BITS> W;
+    typedef typename Products<T, HALF>::key K;
+    typedef typename Products<T, HALF>::value V;
     const int li = lane & 15, g = lane >> 4;
+    // (a scale operand shifted left by one has the byte on top; what lies below it decides nothing)
+    auto meet = [&](float sc) {
+        const unsigned y = __float_as_uint(sc) << 1;
+        least = min(least, y - (28u << 24));
+        most = max(most, y);
+    };
+    if constexpr (KvElem<K>::code == DT_F16)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) meet(((r.ks >> (8 * b)) & 255u) >= 228u ? 0.f : scale_of(r.ks, b));       // (not a number: one in either type)
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-        *(bf16x8*)(buf + (w * NB + j) * 1024 + lane * 16) =
-            decode8<BITS>(&r.k[j * BITS / 4], scale_of(r.ks, NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2));
+        *(typename Half16<K>::v8*)(buf + (w * NB + j) * 1024 + lane * 16) =
+            decode8<BITS, K>(&r.k[j * BITS / 4], scale_of(r.ks, NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2));
     if (NB == 1 && (w & 1)) return;
-    const int block = NB == 1 ? 0 : NB == 2 ? li >> 3 : li >> 2;
+    const int block = NB == 1 ? 0 : NB == 2 ? li >> 3 : NB == 3 ? min(li, 11) >> 2 : li >> 2;
     if (edge) {
         unsigned part = 0;                                         // byte b, bit i: row v_row(g, i) is not finite in block b
 #pragma unroll
@@ -742,14 +788,17 @@ template <int NB, int BITS> __device__ __forceinline__ void wide_convert(WideTil
     }
     float sc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sc[i] = scale_of(r.vs[i], block);
+    for (int i = 0; i < 8; ++i) {
+        sc[i] = scale_of(r.vs[i], block);
+        if constexpr (HALF) meet(sc[i]);
+    }
     unsigned char* to = buf + (4 * NB + (w >> 1) * W::DV + (w & 1) * 2 * W::PW) * 1024 + lane * 16;
 #pragma unroll
     for (int j = 0; j < W::PW; ++j) {
         u32x4 vf[2];
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-            const unsigned a = decode_pair<BITS>(r.v[i], j, sc[i]), b = decode_pair<BITS>(r.v[i + 1], j, sc[i + 1]);
+            const unsigned a = decode_pair<BITS, V>(r.v[i], j, sc[i]), b = decode_pair<BITS, V>(r.v[i + 1], j, sc[i + 1]);
             vf[0][i >> 1] = __builtin_amdgcn_perm(b, a, 0x05040100u);
             vf[1][i >> 1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
         }
@@ -758,43 +807,34 @@ template <int NB, int BITS> __device__ __forceinline__ void wide_convert(WideTil
     }
 }
 
-template <int NB, int BITS, typename T, int QT>
-__global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a) {
-    constexpr int DV = RawTile<NB, BITS>::DV, NQ = AttnTerms<T>::q, NP = AttnTerms<T>::p;
+// a workgroup's walk over its keys; true: a block does not fit the fp16 operands, the state is void (the same for all threads)
+template <int NB, int BITS, typename T, int QT, bool HALF>
+__device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSource& src, const KeyRange& kr, const KeyRange& own, int start, int stop, int i, int h,
+                                          const int (&col)[QT], const int (&lo)[QT], const int (&hi)[QT], WaveState<NB, BITS, T, QT>& st, unsigned char* lds,
+                                          int lane, int w) {
+    typedef Products<T, HALF> P;
+    typedef Half16<typename P::key> HK;
+    typedef Half16<typename P::value> HV;
     typedef WideTile<NB, BITS> W;
-    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int li = lane & 15, g = lane >> 4;
-    const int U = a.g.n * a.g.H;
-    const int u = blockIdx.x % U, rest = blockIdx.x / U;           // (row, head) fastest, then column groups from the last on, then splits
-    const int cg = a.CG - 1 - rest % a.CG, sp = rest / a.CG;
-    const int i = u / a.g.H, h = u - i * a.g.H;
-    const KvRow r = kv_row(a.g, i);
-    const int all0 = cg * 64 * QT, c0 = all0 + w * 16 * QT;
-    const KeyRange kr = key_range(a, r, all0, min(all0 + 64 * QT, a.N) - 1);
-    const int start = (kr.beg & ~31) + sp * a.chunk, stop = min(kr.end, start + a.chunk);
-    if (sp > 0 && start >= stop) return;
-    const KeyRange own = c0 < a.N ? key_range(a, r, c0, min(c0 + 16 * QT, a.N) - 1) : KeyRange{0, 0, -1, 0};
-    int lo[QT], hi[QT], col[QT];
-    lane_columns<QT>(a, r, c0, li, col, lo, hi);
-    bf16x8 qf[QT][NQ][NB];
-    load_queries<NB, T, QT>(a, i, h, col, g, qf);
-    TileSource src;
-    {
-        const long e = max(r.e, 0);
-        src.k = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
-        src.v = src.k + a.g.ckv;
-        src.ks = a.g.scales + e * a.g.se + (long)h * a.g.sh;
-        src.vs = src.ks + a.g.skv;
-    }
-    WaveState<NB, BITS, T, QT> st;
+    constexpr int DV = RawTile<NB, BITS>::DV, NQ = P::q, NP = P::p;
+    const int g = lane >> 4;
+    typename HK::v8 qf[QT][NQ][NB];
+    load_queries<NB, T, QT, HALF>(a, i, h, col, g, qf);
     st.reset();
     float mark[QT] = {};
+    f32x4 lsum[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) lsum[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    typename HV::v8 ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ones[e] = (typename P::value)1.f;
+    unsigned least = ~0u;
+    unsigned most = 0;
     auto edge = [&](int k0) { return k0 + 63 > kr.hi_all || k0 + 64 > stop || k0 < kr.lo_all; };
     WideTile<NB, BITS> raw;
     if (start < stop) {
         wide_load<NB, BITS>(raw, src, start, stop - start, lane, w);
-        wide_convert<NB, BITS>(raw, lds, edge(start), lane, w);
+        wide_convert<NB, BITS, T, HALF>(raw, lds, edge(start), least, most, lane, w);
         if (start + 64 < stop) wide_load<NB, BITS>(raw, src, start + 64, stop - start - 64, lane, w);
     }
     __syncthreads();
@@ -803,7 +843,7 @@ __global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a
         const unsigned char* buf = lds + at * W::bytes;
         const bool work = k0 < own.end && k0 + 64 > own.beg;       // somebody in this wave sees a key of the tile
         const bool more = k0 + 64 < stop;
-        bf16x8 pf[2][QT][NP];
+        typename HV::v8 pf[2][QT][NP];
         if (work) {
             f32x4 s[QT][4];
 #pragma unroll
@@ -817,30 +857,35 @@ __global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a
                 for (int j = 0; j < NB; ++j)
 #pragma unroll
                     for (int hh = 0; hh < 4; ++hh) {
-                        const bf16x8 kf = *(const bf16x8*)(buf + (hh * NB + j) * 1024 + lane * 16);
+                        const typename HK::v8 kf = *(const typename HK::v8*)(buf + (hh * NB + j) * 1024 + lane * 16);
 #pragma unroll
-                        for (int t = 0; t < QT; ++t) s[t][hh] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[t][n][j], s[t][hh], 0, 0, 0);
+                        for (int t = 0; t < QT; ++t) s[t][hh] = HK::mfma32(kf, qf[t][n][j], s[t][hh]);
                     }
             const bool masked = k0 + 63 > own.hi_all || k0 + 64 > stop || k0 < own.lo_all;
-            tile_weights<NB, BITS, T, QT, 2>(s, st, pf, k0, masked, lo, hi, a.c, lane);
+            tile_weights<NB, BITS, T, QT, 2, HALF>(s, st, pf, lsum, k0, masked, lo, hi, a.c, lane);
         }
         if (more) {                                                // the next tile into the other buffer, the one behind it on its way
-            wide_convert<NB, BITS>(raw, lds + (at ^ 1) * W::bytes, edge(k0 + 64), lane, w);
+            wide_convert<NB, BITS, T, HALF>(raw, lds + (at ^ 1) * W::bytes, edge(k0 + 64), least, most, lane, w);
             if (k0 + 128 < stop) wide_load<NB, BITS>(raw, src, k0 + 128, stop - k0 - 128, lane, w);
         }
         if (work) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int x = 0; x < 2; ++x) {
+                if constexpr (kSumByProduct<T, HALF>)
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) lsum[t] = HV::mfma32(ones, pf[x][t][0], lsum[t]);
 #pragma unroll
                 for (int j = 0; j < DV; j += 2) {
-                    const bf16x8 vf[2] = {*(const bf16x8*)(buf + (4 * NB + x * DV + j) * 1024 + lane * 16), *(const bf16x8*)(buf + (4 * NB + x * DV + j + 1) * 1024 + lane * 16)};
+                    const typename HV::v8 vf[2] = {*(const typename HV::v8*)(buf + (4 * NB + x * DV + j) * 1024 + lane * 16),
+                                                   *(const typename HV::v8*)(buf + (4 * NB + x * DV + j + 1) * 1024 + lane * 16)};
 #pragma unroll
                     for (int n = NP - 1; n >= 0; --n)
 #pragma unroll
                         for (int t = 0; t < QT; ++t)
 #pragma unroll
-                            for (int o = 0; o < 2; ++o) st.acc[t][j + o] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[o], pf[x][t][n], st.acc[t][j + o], 0, 0, 0);
+                            for (int o = 0; o < 2; ++o) st.acc[t][j + o] = HV::mfma32(vf[o], pf[x][t][n], st.acc[t][j + o]);
                 }
+            }
             if (edge(k0)) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -856,12 +901,49 @@ __global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a
         }
         __syncthreads();
     }
+    if constexpr (HALF) {
+        constexpr int lo_byte = BITS == 4 ? 127 - 23 : 127 - 15, hi_byte = BITS == 4 ? 127 + 13 : 127 + 7;
+        if (__syncthreads_or(least < (lo_byte - 28u) << 24 || most >= (hi_byte + 1u) << 24)) return true;
+    }
+    const float down = HALF ? __builtin_amdgcn_exp2f(-P::lift) : 1.f;       // (exact: splits of one column may be of either kind)
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        st.l[t] = rows_sum(st.l[t]);
+        st.l[t] = (kSumByProduct<T, HALF> ? lsum[t][0] : rows_sum(st.l[t])) * down;      // (the product's sum is over all keys already)
 #pragma unroll
-        for (int j = 0; j < DV; ++j) st.acc[t][j] += mark[t];
+        for (int j = 0; j < DV; ++j) st.acc[t][j] = st.acc[t][j] * down + mark[t];
     }
+    return false;
+}
+
+template <int NB, int BITS, typename T, int QT>
+__global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, g = lane >> 4;
+    const int U = a.g.n * a.g.H;
+    const int u = blockIdx.x % U, rest = blockIdx.x / U;           // (row, head) fastest, then column groups from the last on, then splits
+    const int cg = a.CG - 1 - rest % a.CG, sp = rest / a.CG;
+    const int i = u / a.g.H, h = u - i * a.g.H;
+    const KvRow r = kv_row(a.g, i);
+    const int all0 = cg * 64 * QT, c0 = all0 + w * 16 * QT;
+    const KeyRange kr = key_range(a, r, all0, min(all0 + 64 * QT, a.N) - 1);
+    const int start = (kr.beg & ~31) + sp * a.chunk, stop = min(kr.end, start + a.chunk);
+    if (sp > 0 && start >= stop) return;
+    const KeyRange own = c0 < a.N ? key_range(a, r, c0, min(c0 + 16 * QT, a.N) - 1) : KeyRange{0, 0, -1, 0};
+    int lo[QT], hi[QT], col[QT];
+    lane_columns<QT>(a, r, c0, li, col, lo, hi);
+    TileSource src;
+    {
+        const long e = max(r.e, 0);
+        src.k = a.g.codes + e * a.g.ce + (long)h * a.g.ch;
+        src.v = src.k + a.g.ckv;
+        src.ks = a.g.scales + e * a.g.se + (long)h * a.g.sh;
+        src.vs = src.ks + a.g.skv;
+    }
+    WaveState<NB, BITS, T, QT> st;
+    bool again = true;
+    if constexpr (sizeof(T) == 2) again = wide_walk<NB, BITS, T, QT, true>(a, src, kr, own, start, stop, i, h, col, lo, hi, st, lds, lane, w);
+    if (again) wide_walk<NB, BITS, T, QT, false>(a, src, kr, own, start, stop, i, h, col, lo, hi, st, lds, lane, w);
     store_columns<NB, BITS, T, QT>(a, st, u, i, h, sp, col, lo, hi, g);
 }
 
@@ -1236,7 +1318,11 @@ int launch_qt(const AttnCacheArgs& a, int qt, unsigned blocks, hipStream_t s) {
         else hipLaunchKernelGGL((attn_cache_vector_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
         return OTTER_OK;
     }
-    if (a.wide) return qt == 1 ? launch_wide<NB, BITS, T, 1>(a, blocks, s) : launch_wide<NB, BITS, T, 2>(a, blocks, s);
+    if (a.wide) {
+        if constexpr (wide_columns(KvElem<T>::code, NB) == 2)
+            if (qt == 2) return launch_wide<NB, BITS, T, 2>(a, blocks, s);
+        return launch_wide<NB, BITS, T, 1>(a, blocks, s);
+    }
     if (qt == 1) hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 1>), dim3(blocks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
     return OTTER_OK;

@@ -82,7 +82,9 @@ def attend(q, k, v, pos, count, causal, window, max_len, scale):
 
 
 def tolerance(out, a_, b_, dtype):
-    """|kernel - out| at most this: both sums (numerator and denominator) carry the relative error of p, the numerator's terms the
-    cut of p to two bf16 terms (2^-17) for 16-bit types and three (2^-24) for fp32; then one rounding to the type."""
-    cut = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -17
+    """|kernel - out| at most this: both sums (numerator and denominator) carry the relative error of p; the numerator's terms are
+    also rounded to matrix operands, by at most half a step of the last one: bf16 activations one fp16 number (2^-11) or two bf16
+    ones (2^-8 2^-8), fp16 activations two fp16 (2^-11 2^-11) or two bf16 ones, fp32 three bf16 ones (2^-24).  Then one rounding to
+    the type.  (A bf16 output's own half step is 2^-8.)"""
+    cut = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -11, torch.float16: 2.0 ** -16}[dtype]
     return a_ * (2 * b_ + cut) * 1.01 + out.abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).tiny

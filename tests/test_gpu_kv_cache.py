@@ -287,6 +287,32 @@ def test_not_a_number_in_masked_places(dev, dtype, t, heads):
     assert torch.equal(got[:, :-1], want[:, :-1]) and bool(torch.isnan(got[:, -1]).all())
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,heads,kv_heads", [(1, 2, 2), (1, 8, 2), (50, 2, 2), (200, 4, 2)])
+@pytest.mark.parametrize("power", [-60, -22, -12, 8, 12, 30])
+def test_values_of_any_magnitude(dev, bits, dtype, t, heads, kv_heads, power):
+    """Value blocks (and, at the small powers, key blocks) whose scales leave the range of one operand type or another: all of
+    them, and single rows among ordinary ones."""
+    from otter_amd import ops
+    d, s, n = 64, 260, 2
+    pos = [s - t, 0]
+    x = _randn(27, 2, n, kv_heads, s, d)
+    x[1, 0] *= 2.0 ** power                                                     # episode 0: every value
+    x[1, 1, :, 3::17] *= 2.0 ** power                                           # episode 1: some rows
+    if power < 0:
+        x[0, 1, :, 2::19] *= 2.0 ** power
+    codes, scales = P.quantise(x, bits)
+    k, v = P.dequantise(codes, scales, bits)
+    q = _randn(28, n, t, heads, d).to(dtype)
+    got = ops.attn_cache(q.to(dev), codes.to(dev), scales.to(dev), _i32(pos, dev))
+    for i in range(n):
+        out, a_, b_ = P.attend(q[i], k[i], v[i], pos[i], t, True, 0, s, d ** -0.5)
+        tol = P.tolerance(out, a_, b_, dtype)
+        fits = out.abs() <= torch.finfo(dtype).max * 0.999
+        assert bool(((got[i].double().cpu() - out).abs() <= tol)[fits].all())
+
+
 # ---------------------------------------------------------------------------------------------------- append and attend in one call
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dtype", DTYPES)
