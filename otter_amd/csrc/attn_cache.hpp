@@ -70,9 +70,11 @@ template <> struct Products<_Float16, true> { typedef _Float16 key, value; stati
 // With one term a weight its sum is one more product, with a row of ones: 16 matrix cycles for 8 weights a lane where additions take 32.
 template <typename T, bool HALF> constexpr bool kSumByProduct = HALF && Products<T, HALF>::p == 1;
 
-// most columns (in units of 16) that a wave of the wide form takes: with 96 or 128 numbers a head and several terms a query, 32 do
-// not fit the registers
-constexpr int wide_columns(int dtype, int nb) { return nb <= 2 || dtype == DT_BF16 ? 2 : 1; }
+// most columns (in units of 16) that a wave of the wide form takes.  Each tile's operands are read from the LDS once for all of
+// them, so 32 are faster wherever their accumulators leave room for the queries' terms: 8 windows of 2047 steps, 12 heads of 64,
+// fp16 136 us against 148 with 16.  fp32 queries are three terms: 174 with 16 against 218 with 32 (spilled); so are 96 or 128
+// numbers a head of fp16.
+constexpr int wide_columns(int dtype, int nb) { return dtype == DT_BF16 || (dtype == DT_F16 && nb <= 2) ? 2 : 1; }
 
 // host: instantiated per element type (attn_cache_*.hip)
 template <typename T> int otter_attn_cache_launch(const AttnCacheArgs& a, int nb, int bits, int qt, unsigned blocks, hipStream_t s);
@@ -915,8 +917,10 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
     return false;
 }
 
+// Three waves a SIMD where a head is at most 64 numbers (170 registers hold a wave's state then): 8 windows of 2047 steps, 12 heads of
+// 64, bf16 123 -> 112 us, fp16 152 -> 136, against two.
 template <int NB, int BITS, typename T, int QT>
-__global__ __launch_bounds__(256, 2) void attn_cache_wide_kernel(AttnCacheArgs a) {
+__global__ __launch_bounds__(256, (NB <= 2 ? 3 : 2)) void attn_cache_wide_kernel(AttnCacheArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g = lane >> 4;
