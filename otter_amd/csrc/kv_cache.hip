@@ -12,7 +12,7 @@ namespace {
 // pieces whose loads are requested together, and the four scale bytes of a row leave in one store.
 template <int NB> struct RowLanes { static constexpr int P = NB == 1 ? 4 : NB == 2 ? 8 : 16, live = 4 * NB; };
 
-template <int NB, int BITS, typename T, int M>
+template <int NB, int BITS, typename T, int M, int MH>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvGeom g, KvOperand<const T> k, KvOperand<const T> v, int vec) {
     constexpr int P = RowLanes<NB>::P, RB = 4 * NB * BITS;
     const int kv = blockIdx.y;
@@ -20,19 +20,18 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvGeom g, KvOperand<const
     const int p = threadIdx.x % P;
     for (int i = blockIdx.z; i < g.n; i += gridDim.z) {
         const KvRow r = kv_row(g, i);
-        float x[M][8];
+        typename KvEight<T>::v8 raw[M];                             // (turned into floats only when all are requested)
         int h[M], at[M];
         bool live[M];
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            const int unit = (blockIdx.x * M + m) * (256 / P) + (int)threadIdx.x / P;
-            h[m] = unit / g.T;
-            const int t = unit - h[m] * g.T;
+            const int unit = (blockIdx.x * (M / MH) + m / MH) * (256 / P) + (int)threadIdx.x / P, group = unit / g.T;
+            const int t = unit - group * g.T;
+            h[m] = group * MH + m % MH;
             at[m] = r.pos + t;
             live[m] = p < RowLanes<NB>::live && h[m] < g.H && r.e >= 0 && t < r.cnt && at[m] >= 0 && at[m] < g.S;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[m][e] = 0.f;
-            if (live[m]) kv_load8<T>(o.p + (long)i * o.row + (long)t * o.step + (long)h[m] * o.head + 8 * p, vec, x[m]);
+            raw[m] = (T)0.f;
+            if (live[m]) kv_fetch8<T>(o.p + (long)i * o.row + (long)t * o.step + (long)h[m] * o.head + 8 * p, vec, raw[m]);
         }
         if (g.idx && r.e >= 0 && i + 1 < g.n) {                     // an episode listed twice: the last listing is the one that is written
             bool later = false;
@@ -41,9 +40,12 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvGeom g, KvOperand<const
         }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            const unsigned sb = kv_scale_byte<BITS>(kv_block_top(x[m]));
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (float)raw[m][e];
+            const unsigned sb = kv_scale_byte<BITS>(kv_block_top(x));
             unsigned w[BITS / 4];
-            kv_encode8<BITS>(x[m], sb, w);
+            kv_encode8<BITS>(x, sb, w);
             unsigned word = sb;                                     // the row's scale bytes, gathered in its first lane
             if constexpr (NB >= 2) word |= __shfl_down(sb, 4, P) << 8;
             if constexpr (NB >= 3) word |= __shfl_down(sb, 8, P) << 16;
@@ -64,34 +66,36 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvGeom g, KvOperand<const
     }
 }
 
-template <int BITS> __device__ __forceinline__ void kv_decode8(const unsigned (&w)[BITS / 4], unsigned scale_byte, float (&x)[8]) {
-    const float sc = __uint_as_float(scale_byte << 23);
+// eight codes -> numbers; the first and the last four with a scale of their own
+template <int BITS> __device__ __forceinline__ void kv_decode8(const unsigned (&w)[BITS / 4], const unsigned (&scale_byte)[2], float (&x)[8]) {
+    const float s0 = __uint_as_float(scale_byte[0] << 23), s1 = __uint_as_float(scale_byte[1] << 23);
     f32x2 y[4];
     if constexpr (BITS == 4) {
-        y[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 0);
-        y[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 1);
-        y[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 2);
-        y[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], sc, 3);
+        y[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s0, 0);
+        y[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s0, 1);
+        y[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s1, 2);
+        y[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[0], s1, 3);
     } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            y[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[h], sc, false);
-            y[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[h], sc, true);
+            y[2 * h] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[h], h ? s1 : s0, false);
+            y[2 * h + 1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(w[h], h ? s1 : s0, true);
         }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = y[i >> 1][i & 1];
 }
 
-template <typename T> __device__ __forceinline__ void kv_store8(T* p, bool vec, const float (&x)[8]) {
+// `second`: where the last four of the eight go (4 = behind the first)
+template <typename T> __device__ __forceinline__ void kv_store8(T* p, bool vec, const float (&x)[8], int second) {
     if constexpr (sizeof(T) == 4) {
         if (vec) {
             *(f32x4*)p = (f32x4){x[0], x[1], x[2], x[3]};
-            *(f32x4*)(p + 4) = (f32x4){x[4], x[5], x[6], x[7]};
+            *(f32x4*)(p + second) = (f32x4){x[4], x[5], x[6], x[7]};
             return;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = x[i];
+        for (int i = 0; i < 8; ++i) p[(i & 4 ? second - 4 : 0) + i] = x[i];
     } else {
         typename Half16<T>::v8 o;
 #pragma unroll
@@ -103,39 +107,51 @@ template <typename T> __device__ __forceinline__ void kv_store8(T* p, bool vec, 
     }
 }
 
-template <int NB, int BITS, typename T, int M>
+// A lane's eight numbers are neighbours in 16 bits; in fp32 it takes four of the row's first half and four of its second, so that each
+// of its two 16-byte stores fills whole lines with its neighbours' (64 x 1500 steps x 6 heads of 64, 4 bits -> fp32 78 us against 91).
+template <int NB, int BITS, typename T, int M, int MH>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvGeom g, KvOperand<T> k, KvOperand<T> v, int vec) {
-    constexpr int P = RowLanes<NB>::P, RB = 4 * NB * BITS;
+    constexpr int P = RowLanes<NB>::P, RB = 4 * NB * BITS, NUM = sizeof(T) == 4 ? 4 : 8, HALF = sizeof(T) == 4 ? 16 * NB : 4;
     const int kv = blockIdx.y;
     const KvOperand<T>& o = kv ? v : k;
     const int p = threadIdx.x % P;
     if (p >= RowLanes<NB>::live) return;
     for (int i = blockIdx.z; i < g.n; i += gridDim.z) {
         const KvRow r = kv_row(g, i);
-        unsigned w[M][BITS / 4], sb[M];
+        unsigned w[M][BITS / 4], sb[M][2];
         int h[M], t[M];
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            const int unit = (blockIdx.x * M + m) * (256 / P) + (int)threadIdx.x / P;
-            h[m] = unit / g.T;
-            t[m] = unit - h[m] * g.T;
+            const int unit = (blockIdx.x * (M / MH) + m / MH) * (256 / P) + (int)threadIdx.x / P, group = unit / g.T;
+            t[m] = unit - group * g.T;
+            h[m] = group * MH + m % MH;
             const int at = r.pos + t[m];
-            sb[m] = 0;
+            sb[m][0] = sb[m][1] = 0;
 #pragma unroll
             for (int q = 0; q < BITS / 4; ++q) w[m][q] = 0;
             if (h[m] < g.H && r.e >= 0 && t[m] < r.cnt && at >= 0 && at < g.S) {
-                const unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h[m] * g.ch + (long)at * RB + p * BITS;
-                sb[m] = g.scales[kv * g.skv + (long)r.e * g.se + (long)h[m] * g.sh + (long)at * 4 + (p >> 2)];
-                if constexpr (BITS == 4) w[m][0] = *(const unsigned*)c;
-                else { const uint2 u = *(const uint2*)c; w[m][0] = u.x; w[m][1] = u.y; }
+                const unsigned char* c = g.codes + kv * g.ckv + (long)r.e * g.ce + (long)h[m] * g.ch + (long)at * RB + p * (NUM * BITS / 8);
+                const unsigned char* sc = g.scales + kv * g.skv + (long)r.e * g.se + (long)h[m] * g.sh + (long)at * 4;
+                sb[m][0] = sc[p * NUM / 32];
+                if constexpr (NUM == 4) {
+                    sb[m][1] = sc[(HALF + p * 4) / 32];
+                    if constexpr (BITS == 4) w[m][0] = *(const unsigned short*)c | (unsigned)*(const unsigned short*)(c + RB / 2) << 16;
+                    else { w[m][0] = *(const unsigned*)c; w[m][1] = *(const unsigned*)(c + RB / 2); }
+                } else if constexpr (BITS == 4) {
+                    w[m][0] = *(const unsigned*)c;
+                } else {
+                    const uint2 u = *(const uint2*)c;
+                    w[m][0] = u.x; w[m][1] = u.y;
+                }
             }
         }
 #pragma unroll
         for (int m = 0; m < M; ++m) {
             if (h[m] >= g.H) continue;
             float x[8];
+            if constexpr (NUM == 8) sb[m][1] = sb[m][0];
             kv_decode8<BITS>(w[m], sb[m], x);                       // (what does not exist: codes 0, the number 0)
-            kv_store8<T>(o.p + (long)i * o.row + (long)t[m] * o.step + (long)h[m] * o.head + 8 * p, vec, x);
+            kv_store8<T>(o.p + (long)i * o.row + (long)t[m] * o.step + (long)h[m] * o.head + NUM * p, vec, x, HALF);
         }
     }
 }
@@ -145,23 +161,30 @@ inline bool operand_vec(const otter_kv_operand* o, int dtype) {
     return aligned16(o->p) && (o->row * es) % 16 == 0 && (o->step * es) % 16 == 0 && (o->head * es) % 16 == 0;
 }
 
-template <bool WRITE, int NB, int BITS, typename T, int M>
+template <bool WRITE, int NB, int BITS, typename T, int M, int MH>
 void launch_m(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
-    const long rows = (long)g.H * g.T, a_block = M * (256 / RowLanes<NB>::P);
+    const long rows = (long)(g.H / MH) * g.T, a_block = M / MH * (256 / RowLanes<NB>::P);
     const dim3 grid((unsigned)((rows + a_block - 1) / a_block), 2, (unsigned)std::min(g.n, 65535));
     if constexpr (WRITE)
-        hipLaunchKernelGGL((kv_write_kernel<NB, BITS, T, M>), grid, dim3(256), 0, s, g, (KvOperand<const T>{(const T*)k->p, k->row, k->step, k->head}),
+        hipLaunchKernelGGL((kv_write_kernel<NB, BITS, T, M, MH>), grid, dim3(256), 0, s, g, (KvOperand<const T>{(const T*)k->p, k->row, k->step, k->head}),
                            (KvOperand<const T>{(const T*)v->p, v->row, v->step, v->head}), vec);
     else
-        hipLaunchKernelGGL((kv_read_kernel<NB, BITS, T, M>), grid, dim3(256), 0, s, g, (KvOperand<T>{(T*)k->p, k->row, k->step, k->head}),
+        hipLaunchKernelGGL((kv_read_kernel<NB, BITS, T, M, MH>), grid, dim3(256), 0, s, g, (KvOperand<T>{(T*)k->p, k->row, k->step, k->head}),
                            (KvOperand<T>{(T*)v->p, v->row, v->step, v->head}), vec);
 }
 
-// one piece a lane while that leaves the chip short of workgroups, four otherwise
+// One piece a lane while that leaves the chip short of workgroups, four otherwise.  A wave that writes takes the same four rows of
+// four heads where the heads allow: it reads runs of four heads (one projection's output holds q | k | v of a step, so a head alone
+// is 256 bytes of 6 KB): 16 histories of 4093 steps x 8 heads of 128, bf16 -> 4 bits 72 us against 86 with sixteen rows of one head.  Reading
+// is as fast or faster along one head (56 us against 60).
 template <bool WRITE, int NB, int BITS, typename T>
 void launch(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
-    if ((long)g.H * g.T * RowLanes<NB>::P / 1024 * 2 * g.n >= 2048) launch_m<WRITE, NB, BITS, T, 4>(g, k, v, vec, s);
-    else launch_m<WRITE, NB, BITS, T, 1>(g, k, v, vec, s);
+    if ((long)g.H * g.T * RowLanes<NB>::P / 1024 * 2 * g.n >= 2048) {
+        if (WRITE && g.H % 4 == 0) launch_m<WRITE, NB, BITS, T, 4, WRITE ? 4 : 1>(g, k, v, vec, s);
+        else launch_m<WRITE, NB, BITS, T, 4, 1>(g, k, v, vec, s);
+    } else {
+        launch_m<WRITE, NB, BITS, T, 1, 1>(g, k, v, vec, s);
+    }
 }
 
 template <bool WRITE, int BITS, typename T>

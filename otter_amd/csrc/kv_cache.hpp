@@ -97,22 +97,22 @@ template <> struct KvElem<float> { static constexpr int code = DT_F32; };
 template <> struct KvElem<__bf16> { static constexpr int code = DT_BF16; };
 template <> struct KvElem<_Float16> { static constexpr int code = DT_F16; };
 
-// eight consecutive numbers as floats; `vec`: 16-byte aligned
-template <typename T> __device__ __forceinline__ void kv_load8(const T* p, bool vec, float (&x)[8]) {
+// eight consecutive numbers as they lie in memory; `vec`: 16-byte aligned
+template <typename T> struct KvEight { typedef __attribute__((ext_vector_type(8))) T v8; };
+template <typename T> __device__ __forceinline__ void kv_fetch8(const T* p, bool vec, typename KvEight<T>::v8& x) {
     if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
-        } else {
-            const typename Half16<T>::v8 a = *(const typename Half16<T>::v8*)p;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
-        }
+        x = *(const typename KvEight<T>::v8*)__builtin_assume_aligned(p, 16);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)p[i];
+        for (int i = 0; i < 8; ++i) x[i] = p[i];
     }
+}
+// the same as floats
+template <typename T> __device__ __forceinline__ void kv_load8(const T* p, bool vec, float (&x)[8]) {
+    typename KvEight<T>::v8 r;
+    kv_fetch8<T>(p, vec, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)r[i];
 }
 
 template <typename T> struct KvOperand { T* p; long row, step, head; };   // element strides
