@@ -355,7 +355,7 @@ typedef struct otter_kv_rows {
 /* element (i, t, h, d) = p[i*row + t*step + h*head + d], strides in elements; OTTER_DT_* given by the call */
 typedef struct otter_kv_operand { void* p; long row, step, head; } otter_kv_operand;
 
-/* k and v (read only) into the cache.  An episode listed more than once: only its last listing is written. */
+/* k and v (read only) into the cache, whose episodes must not overlap.  An episode listed more than once: only its last listing is written. */
 int otter_kv_cache_write(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* k,
                          const otter_kv_operand* v, void* stream);
 /* the cache's numbers into k and v; rows that do not exist become zeros.  fp16: cut at +-65504. */
@@ -365,10 +365,11 @@ int otter_kv_cache_read(const otter_kv_cache* cache, const otter_kv_rows* rows, 
  * 0 .. x (causal) or 0 .. pos[e] + count[i] - 1 (not causal), of these only the last `window` up to that position (0: all) and
  * only those below max_len (what the caller knows about its lengths; capacity if nothing) and capacity.  A query that sees
  * nothing, and every t >= count[i], gives zeros.  q, out: q_heads heads, a multiple of the cache's; query head j reads key head
- * j / (q_heads / heads).
+ * j / (q_heads / heads).  fp16: cut at +-65504.
  * k_new / v_new (both or none; steps == 1, count NULL): the step's own key and value, quantised, stored at pos[e] and attended to by the
  * same launch -- as otter_kv_cache_write followed by this call.
- * workspace: otter_attn_cache_workspace_floats(...) floats, 8-byte aligned, private to the call until it has run (0: none). */
+ * workspace: otter_attn_cache_workspace_floats(...) floats (max_len there: no more than the capacity), 8-byte aligned, private to
+ * the call until it has run (0: none). */
 long otter_attn_cache_workspace_floats(int dtype, int n_rows, int steps, int q_heads, int kv_heads, int head_dim, int window, int max_len);
 int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows* rows, int dtype, const otter_kv_operand* q, int q_heads,
                      const otter_kv_operand* k_new, const otter_kv_operand* v_new, const otter_kv_operand* out, int causal,

@@ -34,7 +34,7 @@ Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max
         p.nsplit = (int)ceil_div(span, p.chunk);
     }
     const long blocks = p.wide || p.kw == 4 ? items * p.nsplit : p.cg == 1 ? ceil_div(U, 4) : U * ceil_div(p.cg, 4);
-    p.ok = blocks < (1L << 31);
+    p.ok = blocks < (1L << 24);                                     // (a grid has at most 2^32 threads a dimension)
     p.blocks = (unsigned)blocks;
     return p;
 }
@@ -57,7 +57,7 @@ extern "C" int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows
     OTTER_REQUIRE(cache->episodes > 0, OTTER_ERR_INVALID_ARGUMENT, "%s: the cache has no episodes", name);
     OTTER_REQUIRE(q_heads > 0 && q_heads % cache->heads == 0, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: %d query heads over %d key heads", name, q_heads, cache->heads);
     OTTER_REQUIRE(window >= 0 && max_len > 0, OTTER_ERR_INVALID_ARGUMENT, "%s: window=%d max_len=%d", name, window, max_len);
-    OTTER_REQUIRE(scale > 0.f && scale < 3.0e38f, OTTER_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", name);
+    OTTER_REQUIRE(scale > 0.f && scale < 1.0e38f, OTTER_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", name);
     if (int rc = otter_kv_check_operand(q, dtype, false, "q", name)) return rc;
     if (int rc = otter_kv_check_operand(out, dtype, true, "out", name)) return rc;
     const long es = dtype == DT_F32 ? 4 : 2;
@@ -68,6 +68,7 @@ extern "C" int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows
         OTTER_REQUIRE(rows->steps == 1 && !rows->count, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: appends one step to every listed row (steps=%d, no count)", name, rows->steps);
         if (int rc = otter_kv_check_operand(k_new, dtype, false, "k_new", name)) return rc;
         if (int rc = otter_kv_check_operand(v_new, dtype, false, "v_new", name)) return rc;
+        if (int rc = otter_kv_check_writable(cache, name)) return rc;
     }
     const int G = q_heads / cache->heads;
     OTTER_REQUIRE((long)rows->steps * G < (1L << 30) && (long)rows->n_rows * cache->heads < (1L << 30), OTTER_ERR_UNSUPPORTED_SHAPE, "%s: too many rows, heads or steps", name);

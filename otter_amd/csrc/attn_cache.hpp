@@ -353,9 +353,10 @@ __device__ __forceinline__ void tile_values(const RawTile<NB, BITS>& r, WaveStat
     }
 }
 
-// value rows whose block is not finite: zeros in their place, and NaN as the mark of the columns that see one
+// value rows whose block is not finite, and rows before `beg`, which nobody sees: zeros in their place, and NaN as the mark of the columns
+// that see one
 template <int NB, int BITS, typename T, int QT>
-__device__ __forceinline__ void clean_values(RawTile<NB, BITS>& r, float (&mark)[QT], int k0, const int (&lo)[QT], const int (&hi)[QT], int lane) {
+__device__ __forceinline__ void clean_values(RawTile<NB, BITS>& r, float (&mark)[QT], int k0, int beg, const int (&lo)[QT], const int (&hi)[QT], int lane) {
     constexpr int VW = RawTile<NB, BITS>::VW;
     const int li = lane & 15, g = lane >> 4;
     const int acc_block = NB == 1 ? 0 : NB == 2 ? g >> 1 : g, own_block = NB == 1 ? 0 : NB == 2 ? li >> 3 : li >> 2;
@@ -378,7 +379,7 @@ __device__ __forceinline__ void clean_values(RawTile<NB, BITS>& r, float (&mark)
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (((r.vs[i] >> (8 * own_block)) & 255u) >= 228u) {
+        if (((r.vs[i] >> (8 * own_block)) & 255u) >= 228u || k0 + v_row(g, i) < beg) {
             r.vs[i] = 0;
 #pragma unroll
             for (int w = 0; w < VW; ++w) r.v[i][w] = 0;
@@ -487,7 +488,7 @@ __device__ __forceinline__ void store_columns(const AttnCacheArgs& a, const Wave
             } else {
                 typename Half16<T>::v8 v;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = (T)y[e];
+                for (int e = 0; e < 8; ++e) v[e] = kv_result<T>(y[e]);
                 *(typename Half16<T>::v8*)(o + 8 * q) = v;
             }
         }
@@ -639,7 +640,7 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
 #pragma unroll
             for (int i = 0; i < 8; ++i) suspect |= raw.vs[i] & (raw.vs[i] << 1) & (raw.vs[i] << 2) & 0x80808080u;
         }
-        if (__any(suspect != 0)) clean_values<NB, BITS, T, QT>(raw, mark, k0, lo, hi, lane);
+        if (__any(suspect != 0) || k0 < kr.beg) clean_values<NB, BITS, T, QT>(raw, mark, k0, kr.beg, lo, hi, lane);
         tile_values<NB, BITS, T, QT>(raw, st, pf[0], lane);
         if (more) values(k0 + stride);
     }
@@ -695,7 +696,7 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
                 } else {
                     typename Half16<T>::v4 v;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.f : o[e] * inv);
+                    for (int e = 0; e < 4; ++e) v[e] = kv_result<T>(none ? 0.f : o[e] * inv);
                     *(typename Half16<T>::v4*)y = v;
                 }
             } else {
@@ -743,11 +744,12 @@ template <int NB, int BITS> __device__ __forceinline__ void wide_load(WideTile<N
     for (int i = 0; i < 8; ++i) buffer_words<PB>(vc, vl + ((i & 3) + 16 * (i >> 2)) * RB, r.v[i]);
 }
 
-// `edge`: the tile has keys that some column does not see: blocks that are not finite are taken out and named in the masks
+// `edge`: the tile has keys that some column does not see: blocks that are not finite are taken out and named in the masks; so are
+// the tile's first `before` rows, which no column sees
 // `least`, `most`: over the bytes met, as the top bits of a word, `least` less 28: the lowest exponent's byte 27 and the zeros of
 // rows that do not exist wrap around and pass
 template <int NB, int BITS, typename T, bool HALF>
-__device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned char* buf, bool edge, unsigned& least, unsigned& most, int lane, int w) {
+__device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned char* buf, bool edge, int before, unsigned& least, unsigned& most, int lane, int w) {
     typedef WideTile<NB, BITS> W;
     typedef typename Products<T, HALF>::key K;
     typedef typename Products<T, HALF>::value V;
@@ -775,7 +777,7 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
             for (int b = 0; b < NB; ++b) part |= (((r.vs[i] >> (8 * b)) & 255u) >= 228u ? 1u : 0u) << (8 * b + i);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (((r.vs[i] >> (8 * block)) & 255u) >= 228u) r.vs[i] = r.v[i][0] = 0;
+            if (((r.vs[i] >> (8 * block)) & 255u) >= 228u || 32 * (w >> 1) + v_row(g, i) < before) r.vs[i] = r.v[i][0] = 0;
         unsigned rows[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -836,7 +838,7 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
     WideTile<NB, BITS> raw;
     if (start < stop) {
         wide_load<NB, BITS>(raw, src, start, stop - start, lane, w);
-        wide_convert<NB, BITS, T, HALF>(raw, lds, edge(start), least, most, lane, w);
+        wide_convert<NB, BITS, T, HALF>(raw, lds, edge(start), kr.beg - start, least, most, lane, w);
         if (start + 64 < stop) wide_load<NB, BITS>(raw, src, start + 64, stop - start - 64, lane, w);
     }
     __syncthreads();
@@ -867,7 +869,7 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
             tile_weights<NB, BITS, T, QT, 2, HALF>(s, st, pf, lsum, k0, masked, lo, hi, a.c, lane);
         }
         if (more) {                                                // the next tile into the other buffer, the one behind it on its way
-            wide_convert<NB, BITS, T, HALF>(raw, lds + (at ^ 1) * W::bytes, edge(k0 + 64), least, most, lane, w);
+            wide_convert<NB, BITS, T, HALF>(raw, lds + (at ^ 1) * W::bytes, edge(k0 + 64), kr.beg - k0 - 64, least, most, lane, w);
             if (k0 + 128 < stop) wide_load<NB, BITS>(raw, src, k0 + 128, stop - k0 - 128, lane, w);
         }
         if (work) {
@@ -1147,12 +1149,17 @@ __global__ __launch_bounds__(256, (NC == 1 && (BITS == 4 || NB <= 2) ? 4 : NC ==
 #pragma unroll
             for (int c = 0; c < NC; ++c) s[c] = key >= kr.lo_all && key < stop ? s[c] : -INFINITY;
 #pragma unroll
-            for (int q = 0; q < 16; ++q) raw.vs[q] = k0 + 16 * g + q >= kr.lo_all ? raw.vs[q] : 0u;
+            for (int q = 0; q < 16; ++q) {
+                const bool seen = k0 + 16 * g + q >= kr.lo_all;
+                raw.vs[q] = seen ? raw.vs[q] : 0u;
+#pragma unroll
+                for (int x = 0; x < VW; ++x) raw.v[q][x] = seen ? raw.v[q][x] : 0u;
+            }
         }
         float p[NC];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            if (__any(__builtin_fmaf(s[c], a.c, -m[c] * a.c) > 8.f) || m[c] == -INFINITY) {       // (see move_reference)
+            if (__any(__builtin_fmaf(s[c], a.c, -m[c] * a.c) > 8.f) || m[c] == -INFINITY) {       // (see tile_weights)
                 const float mn = fmaxf(m[c], all_max(s[c]));
                 const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[c] - mn) * a.c);
                 m[c] = mn;
@@ -1185,7 +1192,7 @@ __global__ __launch_bounds__(256, (NC == 1 && (BITS == 4 || NB <= 2) ? 4 : NC ==
                 typedef __attribute__((ext_vector_type(DV))) T vt;
                 vt v;
 #pragma unroll
-                for (int j = 0; j < DV; ++j) v[j] = (T)(none ? 0.f : acc[c][j] * inv);
+                for (int j = 0; j < DV; ++j) v[j] = kv_result<T>(none ? 0.f : acc[c][j] * inv);
                 if constexpr (sizeof(vt) <= 16) *(vt*)o = v;
                 else {
                     *(f32x4*)o = (f32x4){v[0], v[1], v[2], v[3]};
@@ -1224,7 +1231,7 @@ __global__ __launch_bounds__(256, (NC == 1 && (BITS == 4 || NB <= 2) ? 4 : NC ==
             } else {
                 typename Half16<T>::v4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.f : o[e] * inv);
+                for (int e = 0; e < 4; ++e) v[e] = kv_result<T>(none ? 0.f : o[e] * inv);
                 *(typename Half16<T>::v4*)y = v;
             }
         } else {
@@ -1296,7 +1303,7 @@ __global__ __launch_bounds__(256) void attn_cache_join_kernel(AttnCacheArgs a, i
     } else {
         typename Half16<T>::v4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(none ? 0.f : o[e] * inv);
+        for (int e = 0; e < 4; ++e) v[e] = kv_result<T>(none ? 0.f : o[e] * inv);
         *(typename Half16<T>::v4*)y = v;
     }
 }

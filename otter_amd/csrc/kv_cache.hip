@@ -99,8 +99,8 @@ template <typename T> __device__ __forceinline__ void kv_store8(T* p, bool vec, 
     } else {
         typename Half16<T>::v8 o;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)                                // exact in bf16; fp16: rounded below 2^-14, cut at its largest number (NaN stays)
-            o[i] = (T)(sizeof(T) == 2 && KvElem<T>::code == DT_F16 && x[i] == x[i] ? __builtin_amdgcn_fmed3f(x[i], -65504.f, 65504.f) : x[i]);
+        for (int i = 0; i < 8; ++i)                                // exact in bf16; fp16: rounded below 2^-14
+            o[i] = kv_result<T>(x[i]);
         if (vec) { *(typename Half16<T>::v8*)p = o; return; }
 #pragma unroll
         for (int i = 0; i < 8; ++i) p[i] = o[i];
@@ -202,6 +202,8 @@ int move(const otter_kv_cache* c, const otter_kv_rows* r, int dtype, const otter
     if (int rc = otter_kv_check_operand(k, dtype, !WRITE, "k", name)) return rc;
     if (int rc = otter_kv_check_operand(v, dtype, !WRITE, "v", name)) return rc;
     OTTER_REQUIRE((long)c->heads * r->steps * 16 < (1L << 31) - 1024, OTTER_ERR_UNSUPPORTED_SHAPE, "%s: %d heads x %d steps too large", name, c->heads, r->steps);
+    if (WRITE)
+        if (int rc = otter_kv_check_writable(c, name)) return rc;
     const KvGeom g = otter_kv_geom(c, r);
     const int vec = operand_vec(k, dtype) && operand_vec(v, dtype), nb = c->head_dim / 32;
     if (c->bits == 4) {
@@ -235,6 +237,15 @@ int otter_kv_check(const otter_kv_cache* c, const otter_kv_rows* r, const char* 
                   OTTER_ERR_INVALID_ARGUMENT, "%s: heads of the cache overlap", name);
     OTTER_REQUIRE(r->n_rows >= 0 && r->steps >= 0 && r->steps <= (1 << 30), OTTER_ERR_INVALID_ARGUMENT, "%s: n_rows=%d steps=%d", name, r->n_rows, r->steps);
     OTTER_REQUIRE(r->idx || r->n_rows <= c->episodes, OTTER_ERR_INVALID_ARGUMENT, "%s: %d rows without idx, cache of %d episodes", name, r->n_rows, c->episodes);
+    return OTTER_OK;
+}
+
+// (reading, episodes may share rows; what is written has rows of its own)
+int otter_kv_check_writable(const otter_kv_cache* c, const char* name) {
+    const long row = (long)c->head_dim * c->bits / 8;
+    OTTER_REQUIRE((c->episodes <= 1 || (c->code_episode >= c->capacity * row && c->scale_episode >= c->capacity * 4L)) &&
+                      c->code_kv >= c->capacity * row && c->scale_kv >= c->capacity * 4L,
+                  OTTER_ERR_INVALID_ARGUMENT, "%s: episodes, or keys and values, of the cache overlap", name);
     return OTTER_OK;
 }
 

@@ -97,6 +97,12 @@ template <> struct KvElem<float> { static constexpr int code = DT_F32; };
 template <> struct KvElem<__bf16> { static constexpr int code = DT_BF16; };
 template <> struct KvElem<_Float16> { static constexpr int code = DT_F16; };
 
+// a result in the type of the activations; fp16: cut at its largest number (NaN stays), as everywhere in this library
+template <typename T> __device__ __forceinline__ T kv_result(float v) {
+    if constexpr (KvElem<T>::code == DT_F16) return (T)(v == v ? __builtin_amdgcn_fmed3f(v, -65504.f, 65504.f) : v);
+    else return (T)v;
+}
+
 // eight consecutive numbers as they lie in memory; `vec`: 16-byte aligned
 template <typename T> struct KvEight { typedef __attribute__((ext_vector_type(8))) T v8; };
 template <typename T> __device__ __forceinline__ void kv_fetch8(const T* p, bool vec, typename KvEight<T>::v8& x) {
@@ -119,5 +125,6 @@ template <typename T> struct KvOperand { T* p; long row, step, head; };   // ele
 
 // host: checks of the C structs shared by every entry point; OTTER_OK or error set
 int otter_kv_check(const otter_kv_cache* c, const otter_kv_rows* r, const char* name);
+int otter_kv_check_writable(const otter_kv_cache* c, const char* name);
 int otter_kv_check_operand(const otter_kv_operand* o, int dtype, bool write, const char* what, const char* name);
 KvGeom otter_kv_geom(const otter_kv_cache* c, const otter_kv_rows* r);

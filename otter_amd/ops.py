@@ -748,7 +748,7 @@ def _attn_cache(q: Tensor, k: Optional[Tensor], v: Optional[Tensor], codes, scal
     if window < 0 or (max_len is not None and max_len < 1):
         raise ValueError(f"{name}: window={window}, max_len={max_len}")
     scale = d ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
+    if not 0.0 < scale < 1.0e38:
         raise ValueError(f"{name}: scale must be positive and finite")
     if max_len is not None and max_len < cap:
         cap = int(max_len)

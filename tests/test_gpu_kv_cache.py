@@ -313,6 +313,42 @@ def test_values_of_any_magnitude(dev, bits, dtype, t, heads, kv_heads, power):
         assert bool(((got[i].double().cpu() - out).abs() <= tol)[fits].all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,heads", [(1, 2), (1, 4), (1, 16), (40, 2), (3, 4), (100, 4)])
+def test_codes_that_are_no_numbers_in_masked_places(dev, dtype, t, heads):
+    """8 bits have codes for NaN, which the writer makes only in blocks whose scale says so.  Memory that nobody has written may
+    hold them with any scale: before the window and behind the end it changes nothing."""
+    from otter_amd import ops
+    bits, d, h, s, n = 8, 96, 2, 420, 3
+    pos, window = [10, 75, 310], 25
+    codes, scales, k, v = _filled(dev, 31, n, h, s, d, bits)
+    q = _randn(32, n, t, heads, d).to(dtype)
+    want = ops.attn_cache(q.to(dev), codes, scales, _i32(pos, dev), window=window)
+    for i in range(n):
+        hidden = torch.ones(s, dtype=torch.bool)
+        hidden[max(0, pos[i] - window + 1):pos[i] + t] = False
+        codes[:, i, :, hidden.to(dev)] = 0x7f if i % 2 else 0xff
+        scales[:, i, :, hidden.to(dev)] = 255 if i == 2 else 130
+    got = ops.attn_cache(q.to(dev), codes, scales, _i32(pos, dev), window=window)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("t,heads", [(1, 2), (1, 8), (20, 2), (100, 2)])
+def test_half_precision_outputs_are_cut(dev, t, heads):
+    """Outputs past fp16's largest number: that number, as a read gives it, with one split of the keys and with several."""
+    from otter_amd import ops
+    for s in (64, 2200):
+        codes, scales = _new(dev, 1, 2, s, 64, 4)
+        codes[:, :, :, :, ::2], codes[:, :, :, :, 1::2] = 0x77, 0xff                    # 6, 6, -6, -6, ...
+        scales[0], scales[1] = 127, 127 + 14
+        q = torch.zeros(1, t, heads, 64, dtype=torch.float16, device=dev)
+        got = ops.attn_cache(q, codes, scales, _i32([s - t], dev))
+        sign = torch.tensor([1.0, 1.0, -1.0, -1.0]).repeat(16)
+        want = (65504.0 * sign).repeat(1, t, heads, 1)
+        want[:, :max(0, t - s)] = 0                                                     # steps before position 0 see nothing
+        assert torch.equal(got.float().cpu(), want)
+
+
 # ---------------------------------------------------------------------------------------------------- append and attend in one call
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("dtype", DTYPES)

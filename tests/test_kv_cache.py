@@ -192,3 +192,20 @@ def test_workspace_covers_every_plan():
         rc = lib.otter_attn_cache(cache, _rows(n_rows=n, steps=steps), dtype, op, hq, None, None, op, 1, window, cap, 0.1, ADDR, need - 1, None)
         _refused(rc, f"workspace of {need} floats")
     assert split > 50
+
+
+def test_overlapping_episodes_are_not_written():
+    """Episodes that share rows (an expanded cache) can be read and attended to, never written."""
+    lib = _lib.load()
+    for bad in (dict(code_episode=0), dict(scale_episode=0), dict(code_kv=0), dict(scale_kv=0), dict(code_episode=16 * 32 - 16)):
+        _refused(lib.otter_kv_cache_write(_cache(**bad), _rows(), 2, _operand(), _operand(), None), "overlap")
+        _refused(lib.otter_attn_cache(_cache(**bad), _rows(), 2, _operand(), 2, _operand(), _operand(), _operand(), 1, 0, 16, 0.1, None, 0, None), "overlap")
+
+
+def test_attention_refuses_what_no_launch_holds():
+    lib = _lib.load()
+    for scale in (1.0e38, 3.0e38):                                                       # scale log2(e) would leave fp32
+        _refused(lib.otter_attn_cache(_cache(), _rows(), 2, _operand(), 2, None, None, _operand(), 1, 0, 16, scale, None, 0, None), "scale")
+    # 2^26 rows of one head: one workgroup takes four, a grid has 2^32 threads
+    many = _cache(heads=1, episodes=1 << 27)
+    _refused(lib.otter_attn_cache(many, _rows(n_rows=1 << 27), 2, _operand(), 1, None, None, _operand(), 1, 0, 16, 0.1, None, 0, None), "grid")
