@@ -268,14 +268,6 @@ class PolicyDevice:
         t = rows.view(*lead, 3, self.heads, self.dim // self.heads)
         return t.select(-3, 0), t.select(-3, 1), t.select(-3, 2)
 
-    def _positions(self, batch: int, window: int) -> Tensor:
-        """(window, B) int32, row p = position p for every episode."""
-        key = (batch, window)
-        if getattr(self, "_pos_key", None) != key:
-            self._pos_key = key
-            self._pos = torch.arange(window, dtype=torch.int32, device=self.device)[:, None].expand(window, batch).contiguous()
-        return self._pos
-
     def run(self, window: Tensor, cache: list, n_query: int, pos0: int, idx: Optional[Tensor] = None) -> Tensor:
         """Run positions pos0 .. pos0+n_query-1 of every episode; returns the fp32 outputs (B*n_query, dim).
 
@@ -290,6 +282,9 @@ class PolicyDevice:
             raise ValueError("policy.run: idx goes with whole windows and a quantised cache")
         x = ops.add_pe(window, self.pe, n_query, pos0)
         f32 = torch.float32
+        pos = None
+        if n_query != s and isinstance(cache[0], KVCache):
+            pos = torch.full((cache[0].episodes,), pos0, dtype=torch.int32, device=self.device)
         for blk, kv in zip(self.layers, cache):
             h = ops.layernorm(x, *blk.ln1, out_dtype=f32)
             if isinstance(kv, KVCache):
@@ -299,7 +294,7 @@ class PolicyDevice:
                     kv.write(k, v, idx=idx)
                     a = kv.attend(q, idx=idx, max_len=s).view(b * s, self.dim)
                 else:
-                    a = kv.step(*self._qkv(fresh, b), self._positions(b, s)[pos0], max_len=pos0 + 1).view(b, self.dim)
+                    a = kv.step(*self._qkv(fresh, b), pos, max_len=pos0 + 1).view(b, self.dim)
             else:
                 out = kv.view(b * s, 3 * self.dim) if n_query == s else kv[:, pos0, :]      # (one position: rows strided by S*3*dim)
                 ops.gemm(h, blk.wqkv, blk.n_qkv, blk.bqkv, out=out)

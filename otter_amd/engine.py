@@ -84,8 +84,8 @@ class BatchedRollout:
     batch with no gather; a mixed step runs the two groups one after the other on their own rows.  ``reset(ids)`` of a
     subset therefore never takes the K/V cache away from the other episodes.
 
-    ``kv_bits`` = 4 or 8 keeps the history quantised (:class:`otter_amd.kv_cache.KVCache`): an eighth (a quarter) of the
-    memory, and windows of more than 64 positions; the actions then carry the format's rounding."""
+    ``kv_bits`` = 4 or 8 keeps the history quantised (:class:`otter_amd.kv_cache.KVCache`): an eleventh (a sixth) of
+    the memory, and windows of more than 64 positions; the actions then carry the format's rounding."""
 
     def __init__(self, dev: OtterDevice, n_episodes: int, kv_bits: Optional[int] = None):
         self.dev, self.n, self.kv_bits = dev, int(n_episodes), kv_bits

@@ -1,14 +1,15 @@
 """K/V history held in 4 or 8 bits: the cache object, and its kernels as ``torch.ops.otter_hip.*`` operators.
 
-The policy's fp32 history costs 6 kB a position and layer (q | k | v rows of 768) and its kernels end at 64 positions.  A
+The policy's fp32 history costs 9 kB a position and layer (q | k | v rows of 768) and its kernels end at 64 positions.  A
 :class:`KVCache` holds keys and values only, in blocks of 32 numbers with a power of two as scale: 0.8 kB a position and layer
 in 4 bits (e2m1 codes), 1.6 kB in 8 (e4m3), and histories of any length.  Numbers are quantised as they are written
 (:meth:`KVCache.write`, or :meth:`KVCache.step` together with the attention of a single new position), attended to in that form
 (:meth:`KVCache.attend`), and read back (:meth:`KVCache.read`).  The same cache semantics as ``otter/policy/otter.py:153-175`` /
 ``transformer.py:76-104`` apply: one window per episode, causal attention over the window's earlier positions.
 
-Accuracy is the format's: a 4-bit block is within 1/6 of its largest number (half a step of 2 in 6), an 8-bit one within 2^-4 of
-each number; the arithmetic on the stored numbers is that of the activations' type (fp32 activations: fp32).
+Accuracy is the format's, half a step of the code: a number that is stored in 4 bits is within a fifth of itself if it is at least a
+sixth of its block's largest, in 8 bits within 2^-4 of itself if it is at least 2^-14 of the largest; smaller ones are within a
+quarter of 2^e (2^-10 of 2^e), e the block's exponent.  The arithmetic on the stored numbers is that of the activations' type (fp32 activations: fp32).
 
 | operator | arithmetic |
 |---|---|

@@ -152,3 +152,35 @@ def test_public_objects_take_the_setting(dev):
     pol.refresh()
     assert pol.rollout.kv_bits == 4 and pol.rollout._cache[0].bits == 4
     assert isinstance(BatchedRollout(model.device_model(), 1)._cache[0], torch.Tensor)
+
+
+def test_captured_policy_steps_beside_eager_ones(dev):
+    """A cached step of the policy captured into a graph before any eager one, replayed between eager steps of other batch sizes and positions:
+    every replay gives what the eager step gives on the same history."""
+    model, sd, mc = _model(dev, 8, 59)
+    pol = model.device_model().policy
+    g = torch.Generator().manual_seed(61)
+    windows = {b: torch.randn(b, 8, pol.dim, generator=g).to(dev) for b in (2, 3)}
+    cache, twin, other = (pol.new_cache(b, 8, 4) for b in (2, 2, 3))
+    plain = pol.new_cache(2, 8)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        pol.run(windows[2], plain, 1, 0)                        # (loads the kernels; no quantised cache yet)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = pol.run(windows[2], cache, 1, 1)
+    for turn in range(4):
+        windows[2].copy_(torch.randn(2, 8, pol.dim, generator=g))
+        for c, t in zip(cache, twin):
+            c.codes.zero_(), c.scales.zero_(), t.codes.zero_(), t.scales.zero_()
+        pol.run(windows[2], cache, 1, 0)
+        pol.run(windows[2], twin, 1, 0)
+        pol.run(windows[3], other, 1, turn + 2)
+        graph.replay()
+        want = pol.run(windows[2], twin, 1, 1)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert all(torch.equal(c.codes, t.codes) and torch.equal(c.scales, t.scales) for c, t in zip(cache, twin))
