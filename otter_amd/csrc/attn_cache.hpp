@@ -211,11 +211,10 @@ template <int NP, typename V = __bf16> __device__ __forceinline__ void split_p(c
 #pragma unroll
         for (int n = 0; n < NP; ++n) {
             if constexpr (KvElem<V>::code == DT_F16) {
-                const f16x2 h = {(_Float16)a, (_Float16)b};
-                w[n][i] = __builtin_bit_cast(unsigned, h);
-                if (n + 1 < NP) {
-                    a -= (float)h[0];
-                    b -= (float)h[1];
+                w[n][i] = __builtin_bit_cast(unsigned, (f16x2){(_Float16)a, (_Float16)b});
+                if (n + 1 < NP) {                                  // (one instruction a rest: mixed precision takes either half as it lies)
+                    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel_hi:[1,0,0]" : "+v"(a) : "v"(w[n][i]));
+                    asm("v_fma_mix_f32 %0, %1, -1.0, %0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(b) : "v"(w[n][i]));
                 }
             } else {
                 w[n][i] = pack_bf16(a, b);
