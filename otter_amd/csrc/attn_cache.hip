@@ -9,8 +9,26 @@ struct Plan { int qt, vec, wide, cg, kw, nsplit, chunk; unsigned blocks; bool ok
 
 inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 
-// One step with one or two query heads a key head: the vector form.  Columns otherwise: 16 per wave while all of a row's columns fit, then 32; from 33 on, with several steps, four waves share the
-// converted tiles.
+// Into how many splits the keys of each of `items` workgroups' worth of work are cut.  A compute unit holds R workgroups at a time, and
+// R of them together take R units of time; k < R of them are slower than that (a unit has nothing else to do while they wait for
+// memory), a lone one by `lone`.  Every split of the keys costs `join` of an item (its prologue, its sums written and read again).
+// Measured (one position, 32 / 8 heads of 128, 8000 keys in 4 bits; items: us at 1, 2, 3, 4 splits): 256: 95 67 61 71; 320: 108 77 87 78;
+// 384: 111 85 95 88; 480: 115 126 110 113.  At 640 items of 1000 keys one split takes 21 us, two 26.
+int splits(long items, int R, double lone, double join, long most) {
+    constexpr long units = 256;
+    if (items >= R * units) return 1;
+    int best = 1;
+    double least = 1e30;
+    for (long ns = 1; ns <= std::min<long>(most, 128); ++ns) {
+        const long m = ceil_div(items * ns, units), k = m % R;
+        const double time = ((m - k) + (k ? k + lone * (1.0 - (double)(k - 1) / (R - 1)) : 0.0)) / ns + (ns > 1 ? ns * join * items / units : 0.0);
+        if (time < least) { least = time; best = (int)ns; }
+    }
+    return best;
+}
+
+// One step with one or two query heads a key head: the vector form.  Columns otherwise: 16 per wave while all of a row's columns fit,
+// then 32; from 33 on, with several steps, four waves share the converted tiles.
 // Keys: one wave (wide: one workgroup) walks over all of them while there are enough to fill the chip, four waves and several
 // workgroups share them otherwise.
 Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max_len) {
@@ -27,9 +45,11 @@ Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max
     p.kw = (!p.wide && span > 95 && items < 4096) ? 4 : 1;
     p.nsplit = 1;
     p.chunk = (int)(ceil_div(span, 128) * 128);
-    if (p.kw == 4 || (p.wide && items < 512)) {
-        const long want = ceil_div(p.wide ? 512 : 1024, items), most = ceil_div(span, p.wide ? 512 : 256);
-        const long ns = std::max<long>(1, std::min(want, most));
+    if (p.kw == 4 || p.wide) {
+        // (registers decide how many workgroups a unit holds: the kernels' launch bounds)
+        const int R = p.vec ? (G == 1 ? 4 : 3) : p.wide ? (nb <= 2 ? 3 : 2) : p.qt == 1 ? 3 : 2;
+        const double keys = (double)std::max(span - steps / 2, 1L);                                  // about what the steps see of a causal span
+        const int ns = splits(items, R, p.wide ? 0.35 : 0.75, (p.wide ? 400.0 : 300.0) / keys, ceil_div(span, p.wide ? 512 : 256));
         p.chunk = (int)(ceil_div(ceil_div(span, ns), 128) * 128);
         p.nsplit = (int)ceil_div(span, p.chunk);
     }
