@@ -119,6 +119,7 @@ extern "C" int otter_attn_cache(const otter_kv_cache* cache, const otter_kv_rows
     a.c = scale * 1.44269504088896341f;
     a.vec = p.vec;
     a.wide = p.wide;
+    a.longest = p.wide && p.nsplit == 1 && a.causal && window == 0 && rows->n_rows > 1 && rows->n_rows <= 64;
     a.kw = p.kw;
     a.nsplit = p.nsplit;
     a.chunk = p.chunk;

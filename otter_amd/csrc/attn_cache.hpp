@@ -33,6 +33,7 @@ struct AttnCacheArgs {
     float c;
     int vec;                                        // 1: one step, one or two columns, on the vector unit
     int wide;                                       // 1: four waves x 16 QT columns a workgroup over tiles that they convert together
+    int longest;                                    // wide: 1: (row, column group) pairs in order of their work (causal, no window, at most 64 rows)
     int kw, nsplit, chunk;                          // waves per item along the keys (1 or 4), splits of the key range, keys per split (multiple of 32 * kw)
     float* part;                                    // [nsplit][n * H][N][D + 2] partial sums: D numbers, maximum, sum
 };
@@ -918,6 +919,50 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
     return false;
 }
 
+// The pair (row i, column group cg) that comes at place j when the pairs are in order of how many keys they see, most first.  Histories
+// differ by a factor of three in a batch, and a long one that starts last has the chip to itself: 8 chunks of 500 steps after 2500 to
+// 7600 positions, 32 / 8 heads of 128: 403 us against
+// 540 with the last column groups of all rows first.  Lane = row; a row's groups are
+// first .. first + CG - 1 in units of a group's positions, so the place is found by bisection over that unit, a sum over the wave a step.
+__device__ __forceinline__ int wave_sum_int(int v) {
+    v += __builtin_amdgcn_mov_dpp(v, 0xB1, 0xF, 0xF, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x4E, 0xF, 0xF, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true);
+    v += __builtin_amdgcn_mov_dpp(v, 0x140, 0xF, 0xF, true);
+    const auto a = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    v = (int)(a[0] + a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    return __builtin_amdgcn_readfirstlane((int)(b[0] + b[1]));
+}
+__device__ __forceinline__ KvRow longest_first(const AttnCacheArgs& a, int j, int cols, int lane, int& i, int& cg) {
+    KvRow r = kv_row(a.g, min(lane, a.g.n - 1));
+    const int groups = lane < a.g.n ? a.CG : 0;
+    const int first = r.e >= 0 ? (int)((float)min(max(r.pos, 0), a.max_len) * ((float)a.G / (float)cols)) : 0;
+    if (__ballot(first != __builtin_amdgcn_readfirstlane(first)) == 0) {      // whole windows
+        const int later = j / a.g.n;
+        i = j - later * a.g.n;
+        cg = a.CG - 1 - later;
+    } else {
+        auto above = [&](int t) { return wave_sum_int(min(max(first + a.CG - t, 0), groups)); };      // pairs that see t units or more
+        int t = 0, most = (int)((float)a.max_len * ((float)a.G / (float)cols)) + a.CG + 1;            // above(t) > j >= above(most)
+        while (most - t > 1) {
+            const int mid = t + (most - t) / 2;
+            if (above(mid) > j) t = mid;
+            else most = mid;
+        }
+        j -= above(t + 1);
+        const bool here = groups && first <= t && t < first + a.CG;
+        const unsigned long long rows = __ballot(here);
+        const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(rows >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)rows, 0u));
+        i = __builtin_ctzll(__ballot(here && before == j));
+        cg = t - __builtin_amdgcn_readlane(first, i);
+    }
+    r.e = __builtin_amdgcn_readlane(r.e, i);
+    r.pos = __builtin_amdgcn_readlane(r.pos, i);
+    r.cnt = __builtin_amdgcn_readlane(r.cnt, i);
+    return r;
+}
+
 // Three waves a SIMD where a head is at most 64 numbers (170 registers hold a wave's state then): 8 windows of 2047 steps, 12 heads of
 // 64, bf16 123 -> 112 us, fp16 152 -> 136, against two.
 template <int NB, int BITS, typename T, int QT>
@@ -926,10 +971,25 @@ __global__ __launch_bounds__(256, (NB <= 2 ? 3 : 2)) void attn_cache_wide_kernel
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g = lane >> 4;
     const int U = a.g.n * a.g.H;
-    const int u = blockIdx.x % U, rest = blockIdx.x / U;           // (row, head) fastest, then column groups from the last on, then splits
-    const int cg = a.CG - 1 - rest % a.CG, sp = rest / a.CG;
-    const int i = u / a.g.H, h = u - i * a.g.H;
-    const KvRow r = kv_row(a.g, i);
+    int i, h, cg, sp = 0;
+    KvRow r;
+    if (a.longest) {                                               // head fastest
+        const int j = blockIdx.x / a.g.H;
+        h = blockIdx.x - j * a.g.H;
+        r = longest_first(a, j, 64 * QT, lane, i, cg);
+    } else {                                                       // (row, head) fastest, then column groups from the last on, then splits
+        const int u = blockIdx.x % U, rest = blockIdx.x / U;
+        cg = a.CG - 1 - rest % a.CG;
+        sp = rest / a.CG;
+        i = u / a.g.H;
+        h = u - i * a.g.H;
+        r = kv_row(a.g, i);
+    }
+    // (uniform, which the compiler loses where the two ways meet)
+    i = __builtin_amdgcn_readfirstlane(i);
+    cg = __builtin_amdgcn_readfirstlane(cg);
+    r = {__builtin_amdgcn_readfirstlane(r.e), __builtin_amdgcn_readfirstlane(r.pos), __builtin_amdgcn_readfirstlane(r.cnt)};
+    const int u = i * a.g.H + h;
     const int all0 = cg * 64 * QT, c0 = all0 + w * 16 * QT;
     const KeyRange kr = key_range(a, r, all0, min(all0 + 64 * QT, a.N) - 1);
     const int start = (kr.beg & ~31) + sp * a.chunk, stop = min(kr.end, start + a.chunk);

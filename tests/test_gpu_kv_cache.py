@@ -254,6 +254,23 @@ def test_attend_chunk_after_a_long_history(dev, dtype, bits, d, heads, kv_heads,
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,heads,kv_heads,t", [(2, 3, 3, 150), (17, 7, 1, 40), (63, 2, 2, 130), (64, 4, 2, 129), (65, 2, 2, 130)])
+def test_attend_chunks_after_histories_of_any_length(dev, dtype, n, heads, kv_heads, t):
+    """Workgroups are dealt out by the length of their row's history: none, equal, differing ones, some before the window or past its end,
+    rows that do not exist, short counts; every output of every row is there."""
+    rng = torch.Generator().manual_seed(n)
+    cap = 420
+    pos = torch.randint(0, cap - t + 1, (n,), generator=rng).tolist()
+    _check(dev, 33, 4, dtype, 64, n, t, heads, kv_heads, cap, pos)
+    _check(dev, 34, 8, dtype, 32, n, t, heads, kv_heads, cap, [0] * n)
+    idx = torch.randperm(n, generator=rng).tolist()
+    idx[n // 2], idx[n - 1] = -1, n + 5
+    odd = [(-2000000000, -40, cap - 1, cap + 7, 2000000000)[j % 5] if j % 3 == 0 else p for j, p in enumerate(pos)]
+    count = torch.randint(-1, t + 2, (n,), generator=rng).tolist()
+    _check(dev, 35, 4, dtype, 96, n, t, heads, kv_heads, cap, odd, idx=idx, count=count, max_len=cap - 50)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("t,heads", [(1, 2), (40, 2), (3, 4), (100, 4)])
 def test_not_a_number_in_masked_places(dev, dtype, t, heads):
     """Rows that a query must not see hold NaN (and codes and scales that the writer never makes): before its window, behind its
