@@ -140,7 +140,8 @@ template <int NB, int BITS> __device__ __forceinline__ void load_values(RawTile<
     constexpr int RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, VB = DV * BITS / 8;
     const int li = lane & 15, g = lane >> 4;
     const auto vc = rows_of(src.v, k0, RB, rows), vs = rows_of(src.vs, k0, 4, rows);
-    const int vl = (NB == 3 ? min(li, 11) : li) * VB + 4 * g * RB;  // NB = 3: lanes 12 .. 15 repeat lane 11 (their output rows are not stored)
+    int vl = (NB == 3 ? min(li, 11) : li) * VB + 4 * g * RB;       // NB = 3: lanes 12 .. 15 repeat lane 11 (their output rows are not stored)
+    asm("" : "+v"(vl));                                            // (a sum, not an `or`, of it and a constant goes into the load instruction)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const auto u = __builtin_amdgcn_raw_buffer_load_b128(vs, 16 * g + 64 * h, 0, 0);
@@ -290,18 +291,20 @@ __device__ __forceinline__ void tile_weights(const f32x4 (&s)[QT][2 * NS], WaveS
                     x[u][i] = (key <= hi[t] && key >= lo[t]) ? x[u][i] : -INFINITY;
                 }
         }
-        // (first level by v_med3 with infinity: fmaxf would quiet every score in an instruction of its own first)
-        float mx = -INFINITY;
+        // (by v_med3 with a number above every score: fmaxf would quiet each score in an instruction of its own first)
+        float top[4 * NS];
 #pragma unroll
-        for (int u = 0; u < NS; ++u)
+        for (int k = 0; k < 4 * NS; ++k) top[k] = __builtin_amdgcn_fmed3f(x[k >> 2][2 * (k & 3)], x[k >> 2][2 * (k & 3) + 1], 3.0e38f);
 #pragma unroll
-            for (int i = 0; i < 8; i += 4)
-                mx = fmaxf(mx, fmaxf(__builtin_amdgcn_fmed3f(x[u][i], x[u][i + 1], INFINITY), __builtin_amdgcn_fmed3f(x[u][i + 2], x[u][i + 3], INFINITY)));
+        for (int k = 2 * NS; k > 0; k >>= 1)
+#pragma unroll
+            for (int i = 0; i < k; ++i) top[i] = __builtin_amdgcn_fmed3f(top[i], top[i + k], 3.0e38f);
         // The state moves to a new reference only when a score passes the old one by more than 2^growth (weights then stay below
         // 2^(growth + lift): no precision is lost, the operands have the range): with the running maximum itself some column of 16 moves in most
-        // tiles, and every move costs a multiplication per accumulator.
-        mx = rows_max(mx);
-        if (__any(__builtin_fmaf(mx, c, -st.m[t] * c) > Products<T, HALF>::growth || st.m[t] == -INFINITY)) {
+        // tiles, and every move costs a multiplication per accumulator.  The lanes of a column hold the same reference, so each asks
+        // for its own scores only.
+        if (__any(__builtin_fmaf(top[0], c, -st.m[t] * c) > Products<T, HALF>::growth || st.m[t] == -INFINITY)) {
+            const float mx = rows_max(top[0]);
             const float mn = fmaxf(st.m[t], mx);
             const float corr = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((st.m[t] - mn) * c);
             st.m[t] = mn;
@@ -722,18 +725,21 @@ template <int NB, int BITS> struct WideTile {
     static constexpr int frags = 4 * NB + 2 * DV;                  // operands of 64 lanes x 16 bytes: 4 x 16 keys, then 2 x 32 value rows
     static constexpr int bytes = frags * 1024 + 64;                // and a row mask per (32 keys, block) of the value rows that are not finite
     unsigned k[KW], v[8][1], ks, vs[8];
+    unsigned own;                                                  // value scale word of the key that ks belongs to (range check of the fp16 operands)
 };
 
-template <int NB, int BITS> __device__ __forceinline__ void wide_load(WideTile<NB, BITS>& r, const TileSource& src, int k0, int rows, int lane, int w) {
+template <int NB, int BITS, bool HALF> __device__ __forceinline__ void wide_load(WideTile<NB, BITS>& r, const TileSource& src, int k0, int rows, int lane, int w) {
     constexpr int RB = 4 * NB * BITS, KB = RB / 4, VB = RawTile<NB, BITS>::DV * BITS / 8, PB = WideTile<NB, BITS>::PB;
     const int li = lane & 15, g = lane >> 4;
     const auto kc = rows_of(src.k, k0 + 16 * w, RB, rows - 16 * w), ks = rows_of(src.ks, k0 + 16 * w, 4, rows - 16 * w);
     buffer_words<KB>(kc, li * RB + g * KB, r.k);
     r.ks = __builtin_amdgcn_raw_buffer_load_b32(ks, li * 4, 0, 0);
+    if constexpr (HALF) r.own = __builtin_amdgcn_raw_buffer_load_b32(rows_of(src.vs, k0 + 16 * w, 4, rows - 16 * w), li * 4, 0, 0);
     if (NB == 1 && (w & 1)) return;                                // (one pair a lane: two waves do it)
     const int sub = 32 * (w >> 1);
     const auto vc = rows_of(src.v, k0 + sub, RB, rows - sub), vs = rows_of(src.vs, k0 + sub, 4, rows - sub);
-    const int vl = (NB == 3 ? min(li, 11) : li) * VB + (w & 1) * PB + 4 * g * RB;
+    int vl = (NB == 3 ? min(li, 11) : li) * VB + (w & 1) * PB + 4 * g * RB;
+    asm("" : "+v"(vl));                                            // (see load_values)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const auto u = __builtin_amdgcn_raw_buffer_load_b128(vs, 16 * g + 64 * h, 0, 0);
@@ -746,23 +752,27 @@ template <int NB, int BITS> __device__ __forceinline__ void wide_load(WideTile<N
 
 // `edge`: the tile has keys that some column does not see: blocks that are not finite are taken out and named in the masks; so are
 // the tile's first `before` rows, which no column sees
-// `least`, `most`: over the bytes met, as the top bits of a word, `least` less 28: the lowest exponent's byte 27 and the zeros of
-// rows that do not exist wrap around and pass
+// `least`, `most`: over the scale bytes of the tile's keys (a wave looks at its 16), as the top bits of a word, `least` less 28: the
+// lowest exponent's byte 27 and the zeros of rows that do not exist wrap around and pass
 template <int NB, int BITS, typename T, bool HALF>
 __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned char* buf, bool edge, int before, unsigned& least, unsigned& most, int lane, int w) {
     typedef WideTile<NB, BITS> W;
     typedef typename Products<T, HALF>::key K;
     typedef typename Products<T, HALF>::value V;
     const int li = lane & 15, g = lane >> 4;
-    // (a scale operand shifted left by one has the byte on top; what lies below it decides nothing)
-    auto meet = [&](float sc) {
-        const unsigned y = __float_as_uint(sc) << 1;
-        least = min(least, y - (28u << 24));
-        most = max(most, y);
-    };
-    if constexpr (KvElem<K>::code == DT_F16)
+    auto meet = [&](unsigned word, bool clean) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) meet(((r.ks >> (8 * b)) & 255u) >= 228u ? 0.f : scale_of(r.ks, b));       // (not a number: one in either type)
+        for (int b = 0; b < NB; ++b) {                             // (what lies below the byte decides nothing)
+            const unsigned y = word << (24 - 8 * b);
+            least = min(least, clean && y >= 228u << 24 ? ~0u : y - (28u << 24));
+            most = max(most, clean && y >= 228u << 24 ? 0u : y);
+        }
+    };
+    if constexpr (KvElem<K>::code == DT_F16) meet(r.ks, true);     // (not a number: one in either type)
+    if constexpr (HALF) {                                          // (an edge's rows that are not finite are taken out)
+        if (edge) meet(16 * w + li < before ? 0u : r.own, true);
+        else meet(r.own, false);
+    }
 #pragma unroll
     for (int j = 0; j < NB; ++j)
         *(typename Half16<K>::v8*)(buf + (w * NB + j) * 1024 + lane * 16) =
@@ -792,10 +802,7 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
     }
     float sc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        sc[i] = scale_of(r.vs[i], block);
-        if constexpr (HALF) meet(sc[i]);
-    }
+    for (int i = 0; i < 8; ++i) sc[i] = scale_of(r.vs[i], block);
     unsigned char* to = buf + (4 * NB + (w >> 1) * W::DV + (w & 1) * 2 * W::PW) * 1024 + lane * 16;
 #pragma unroll
     for (int j = 0; j < W::PW; ++j) {
@@ -837,9 +844,9 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
     auto edge = [&](int k0) { return k0 + 63 > kr.hi_all || k0 + 64 > stop || k0 < kr.lo_all; };
     WideTile<NB, BITS> raw;
     if (start < stop) {
-        wide_load<NB, BITS>(raw, src, start, stop - start, lane, w);
+        wide_load<NB, BITS, HALF>(raw, src, start, stop - start, lane, w);
         wide_convert<NB, BITS, T, HALF>(raw, lds, edge(start), kr.beg - start, least, most, lane, w);
-        if (start + 64 < stop) wide_load<NB, BITS>(raw, src, start + 64, stop - start - 64, lane, w);
+        if (start + 64 < stop) wide_load<NB, BITS, HALF>(raw, src, start + 64, stop - start - 64, lane, w);
     }
     __syncthreads();
     int at = 0;
@@ -870,7 +877,7 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
         }
         if (more) {                                                // the next tile into the other buffer, the one behind it on its way
             wide_convert<NB, BITS, T, HALF>(raw, lds + (at ^ 1) * W::bytes, edge(k0 + 64), kr.beg - k0 - 64, least, most, lane, w);
-            if (k0 + 128 < stop) wide_load<NB, BITS>(raw, src, k0 + 128, stop - k0 - 128, lane, w);
+            if (k0 + 128 < stop) wide_load<NB, BITS, HALF>(raw, src, k0 + 128, stop - k0 - 128, lane, w);
         }
         if (work) {
 #pragma unroll
