@@ -558,6 +558,9 @@ __device__ __forceinline__ int append_row(const AttnCacheArgs& a, const KvRow& r
 // (kw = 4), or four items: neighbouring column groups of one (row, head), which read the same rows, or, with one column
 // group, four (row, head) pairs.  (row, head) runs fastest over the workgroups, so that the column groups of one pair meet in
 // one XCD's L2; the last column groups, which see the most keys under a causal mask, start first.
+// Memory-bound where it matters, one position over long histories: 48 rows x 32 / 8 heads of 128 over 7001 to 16383 positions in 4 bits
+// read 610 MB in 126 us (4.8 TB/s, the rate of a large copy), 160 x 16 / 4 heads of 64 over the last 1000 in 8 bits 85 MB in 20 us.
+// Short windows (64 x 8 heads x 32 steps of 96, fp32: 9 us) are one tile a wave: the latency of its dependent loads.
 template <int NB, int BITS, typename T, int QT>
 __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnCacheArgs a) {
     constexpr int D = 32 * NB, RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, NQ = AttnTerms<T>::q;
@@ -636,8 +639,8 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
         bf16x8 pf[1][QT][AttnTerms<T>::p];
         tile_scores<NB, BITS, T, QT>(raw, qf, s, lane);
         if (more) keys(k0 + stride);
-        f32x4 unused[QT];
-        tile_weights<NB, BITS, T, QT, 1>(s, st, pf, unused, k0, masked, lo, hi, a.c, lane);
+        f32x4 unread[QT];                                            // (the sums of products are the wide form's)
+        tile_weights<NB, BITS, T, QT, 1>(s, st, pf, unread, k0, masked, lo, hi, a.c, lane);
         unsigned suspect = 0;
         if (masked) {
 #pragma unroll
@@ -718,6 +721,10 @@ __global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnC
 // convert 64 keys once between them -- a wave its 16 keys and half the numbers of its 32 value rows -- into LDS, in the order in
 // which the matrix operands are read (16 bytes a lane, no conflicts), while the previous tile is being multiplied: two buffers,
 // one barrier a tile.
+// A tile of 64 keys x 32 columns x 64 numbers is 36 products (576 cycles) and 190 vector instructions a wave in bf16, 32 of them
+// exponentials, and the two hardly overlap.  8 windows of 2047 steps, 12 heads of 64, 4 bits: bf16 100 us (820 TFLOP/s of the whole
+// tiles, 512 counting only visible keys), fp16 131, fp32 174; 8 x 500 steps after 2500 to 7600 positions, 32 / 8 heads of 128, bf16
+// 400 us (810 TFLOP/s).  With a kernel of the narrow form the two took 158 and 767 us.
 template <int NB, int BITS> struct WideTile {
     static constexpr int DV = RawTile<NB, BITS>::DV, KW = RawTile<NB, BITS>::KW;
     static constexpr int PW = DV / 4 > 0 ? DV / 4 : 1;             // pairs of numbers of a value row that one wave converts
