@@ -37,7 +37,7 @@ Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max
     p.vec = steps == 1 && G <= 2;
     p.wide = N > 32 && steps > 1;
     // (narrow: 32 only where that leaves two waves a SIMD: few waves are a matter of latency, not of conversions)
-    p.qt = N <= 16 || (p.wide ? N <= 64 || wide_columns(dtype, nb) == 1 : U * ceil_div(N, 32) < 2048) ? 1 : 2;
+    p.qt = N <= 16 || (p.wide ? N <= 64 || wide_columns(dtype, nb) == 1 : U * ceil_div(N, 32) < 2048 || narrow_columns(dtype, nb) == 1) ? 1 : 2;
     const long cols = (p.wide ? 64L : 16L) * p.qt;
     p.cg = (int)ceil_div(N, cols);
     const long span = (window > 0 ? std::min<long>(max_len, (long)window + cols / G + 1) : max_len) + 31;   // keys one item may walk over
@@ -47,7 +47,7 @@ Plan plan(int dtype, int nb, int n, int H, int steps, int G, int window, int max
     p.chunk = (int)(ceil_div(span, 128) * 128);
     if (p.kw == 4 || p.wide) {
         // (registers decide how many workgroups a unit holds: the kernels' launch bounds)
-        const int R = p.vec ? (G == 1 ? 4 : 3) : p.wide ? (nb <= 2 ? 3 : 2) : p.qt == 1 ? 3 : 2;
+        const int R = p.vec ? (G == 1 ? 4 : 3) : p.wide ? (nb <= 2 ? 3 : 2) : narrow_groups(dtype, nb, p.qt);
         const double keys = (double)std::max(span - steps / 2, 1L);                                  // about what the steps see of a causal span
         const int ns = splits(items, R, p.wide ? 0.35 : 0.75, (p.wide ? 400.0 : 300.0) / keys, ceil_div(span, p.wide ? 512 : 256));
         p.chunk = (int)(ceil_div(ceil_div(span, ns), 128) * 128);

@@ -77,6 +77,14 @@ template <typename T, bool HALF> constexpr bool kSumByProduct = HALF && Products
 // numbers a head of fp16.
 constexpr int wide_columns(int dtype, int nb) { return dtype == DT_BF16 || (dtype == DT_F16 && nb <= 2) ? 2 : 1; }
 
+// the same of the narrow form: the three terms of fp32 queries leave no room for 32 with 96 or 128 numbers a head (300 rows x 8 heads
+// of 96 x 32 steps over 300 positions 61 us with 16, 83 with 32; 8 heads of 64 over 1000: 115 and 97)
+constexpr int narrow_columns(int dtype, int nb) { return dtype == DT_F32 && nb > 2 ? 1 : 2; }
+
+// workgroups of the narrow form that a compute unit holds (waves a SIMD): fp32 heads of 128 do not fit the registers of three (one
+// position, 64 rows x 32 / 8 heads over 4096: 69 us with two, 98 with three; heads of 96 fit: 62 with either, 300 x 32 steps 60 against 81)
+constexpr int narrow_groups(int dtype, int nb, int qt) { return qt > 1 || (dtype == DT_F32 && nb == 4) ? 2 : 3; }
+
 // host: instantiated per element type (attn_cache_*.hip)
 template <typename T> int otter_attn_cache_launch(const AttnCacheArgs& a, int nb, int bits, int qt, unsigned blocks, hipStream_t s);
 
@@ -562,7 +570,7 @@ __device__ __forceinline__ int append_row(const AttnCacheArgs& a, const KvRow& r
 // read 610 MB in 126 us (4.8 TB/s, the rate of a large copy), 160 x 16 / 4 heads of 64 over the last 1000 in 8 bits 85 MB in 20 us.
 // Short windows (64 x 8 heads x 32 steps of 96, fp32: 9 us) are one tile a wave: the latency of its dependent loads.
 template <int NB, int BITS, typename T, int QT>
-__global__ __launch_bounds__(256, (QT > 1 ? 2 : 3)) void attn_cache_kernel(AttnCacheArgs a) {
+__global__ __launch_bounds__(256, narrow_groups(KvElem<T>::code, NB, QT)) void attn_cache_kernel(AttnCacheArgs a) {
     constexpr int D = 32 * NB, RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, NQ = AttnTerms<T>::q;
     constexpr int MROW = D + 4;                                    // padded row of the merge buffer
     __shared__ __attribute__((aligned(16))) unsigned char fresh_rows[4][2 * RB + 16];
@@ -1407,8 +1415,12 @@ int launch_qt(const AttnCacheArgs& a, int qt, unsigned blocks, hipStream_t s) {
             if (qt == 2) return launch_wide<NB, BITS, T, 2>(a, blocks, s);
         return launch_wide<NB, BITS, T, 1>(a, blocks, s);
     }
-    if (qt == 1) hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 1>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
+    if constexpr (narrow_columns(KvElem<T>::code, NB) == 2)
+        if (qt == 2) {
+            hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 2>), dim3(blocks), dim3(256), 0, s, a);
+            return OTTER_OK;
+        }
+    hipLaunchKernelGGL((attn_cache_kernel<NB, BITS, T, 1>), dim3(blocks), dim3(256), 0, s, a);
     return OTTER_OK;
 }
 
