@@ -169,6 +169,25 @@ def call_packed(name: str, *args) -> None:
         raise OtterHipError(f"{name} failed (code {rc}): {load().otter_last_error().decode()}")
 
 
+_binding = None
+
+
+def kv_binding():
+    """The compiled way into the K/V-history entry points (``csrc/kv_binding.cpp``), bound to this library's functions."""
+    global _binding
+    if _binding is None:
+        import torch
+        lib = load()
+        try:
+            from . import _kv_binding as b
+        except ImportError as e:
+            raise OtterHipError(f"{os.path.join(_HERE, '_kv_binding.so')} cannot be loaded ({e}): build it with `make -C otter_amd/csrc`") from e
+        names = ("otter_kv_cache_write", "otter_kv_cache_read", "otter_attn_cache", "otter_attn_cache_workspace_floats")
+        b.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in names), torch._C._cuda_getCurrentRawStream)
+        _binding = b
+    return _binding
+
+
 def exported_names():
     return sorted(list(_SIGNATURES) + ["otter_last_error", "otter_hip_abi_version", "otter_grad_stats_workspace_floats",
                                             "otter_pos_emb_packed_elems", "otter_gemm_workspace_floats", "otter_gemm_static_ws_max_n",

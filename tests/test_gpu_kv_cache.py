@@ -485,3 +485,62 @@ def test_offsets_past_32_bits(dev):
         out, a_, b_ = P.attend(x[0, t:t + 1, :h].cpu(), torch.cat([torch.zeros(h, 300, d, dtype=torch.float64), k[0]], 1),
                                torch.cat([torch.zeros(h, 300, d, dtype=torch.float64), v[0]], 1), 300 + t, 1, True, 300, 600, d ** -0.5)
         assert bool(((got[0, t:t + 1].double().cpu() - out).abs() <= P.tolerance(out, a_, b_, torch.float32)).all())
+
+
+def test_the_compiled_way_and_the_other_agree(dev, monkeypatch):
+    """The same calls with the binding and without: equal outputs and caches; ordinary calls are taken by it, refusals raise the same."""
+    from otter_amd import _lib, ops
+
+    class Taken:
+        def __init__(self, inner):
+            self.inner, self.none = inner, 0
+
+        def __getattr__(self, name):
+            def call(*a):
+                got = getattr(self.inner, name)(*a)
+                self.none += got is None
+                return got
+            return call
+
+    class Never:
+        def __getattr__(self, name):
+            return lambda *a: None
+
+    n, t, h, hq, d, cap = 5, 3, 2, 4, 96, 700
+    pos, idx, count = _i32([0, 650, 690, 3, 100, 50], dev), _i32([4, 0, 2, -1, 5], dev), _i32([3, 2, 0, 1, 9], dev)
+    wide = _randn(41, n, t, hq + 2 * h, d).to(dev)
+
+    def run(dtype, bits):
+        codes, scales = _new(dev, 6, h, cap, d, bits)
+        x = wide.to(dtype)
+        q, k, v = x[:, :, :hq], x[:, :, hq:hq + h], x[:, :, hq + h:]
+        ops.kv_cache_write(k, v, codes, scales, pos, idx, count)
+        ops.kv_cache_write(k, v, codes[:, :5], scales[:, :5])
+        out = [*ops.kv_cache_read(codes, scales, d, t, pos, idx, count, dtype=dtype), *ops.kv_cache_read(codes, scales, d, 2), *ops.kv_cache_read(codes, scales, d, 2, n_rows=4)]
+        out += [ops.attn_cache(q, codes, scales, pos, idx, count), ops.attn_cache(q, codes, scales, pos, idx, causal=False, window=9, scale=0.3, max_len=600),
+                ops.attn_cache(q, codes, scales), ops.attn_cache(q[:1, :1], codes, scales, pos, window=1 << 40, max_len=1 << 30)]
+        out += [ops.attn_cache_rows(q[:, 0], k[:, 0], v[:, 0], codes, scales, pos, idx, window=5), ops.attn_cache_rows(q[:, 1], k[:, 1], v[:, 1], codes, scales, scale=1)]
+        return [*out, codes, scales]
+
+    taken = Taken(_lib.kv_binding())
+    for dtype in DTYPES:
+        for bits in (4, 8):
+            monkeypatch.setattr(_lib, "_binding", taken)
+            got = run(dtype, bits)
+            monkeypatch.setattr(_lib, "_binding", Never())
+            want = run(dtype, bits)
+            assert len(got) == len(want) and all(a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b) for a, b in zip(got, want))
+    assert taken.none == 1 * 6                                                   # (the window past 31 bits is left to the other way)
+    monkeypatch.setattr(_lib, "_binding", taken)
+    codes, scales = _new(dev, 2, h, 8, d, 4)
+    q, k = torch.zeros(2, 1, hq, d, device=dev), torch.zeros(2, 1, h, d, device=dev)
+    for call, error in ((lambda: ops.kv_cache_write(k[:, :, :1], k, codes, scales), ValueError), (lambda: ops.kv_cache_write(k, k.half(), codes, scales), TypeError),
+                        (lambda: ops.kv_cache_write(k, k, codes, scales, _i32([0], dev)), ValueError), (lambda: ops.kv_cache_read(codes, scales, 64, 1), ValueError),
+                        (lambda: ops.attn_cache(q, codes, scales, scale=-1.0), ValueError), (lambda: ops.attn_cache(q[:, :, :3], codes, scales), ValueError),
+                        (lambda: ops.attn_cache(q, codes, scales, max_len=0), ValueError), (lambda: ops.attn_cache(q, codes, scales, window=-1), ValueError),
+                        (lambda: ops.kv_cache_write(k, k, codes[:, :1].expand(-1, 2, -1, -1, -1), scales[:, :1].expand(-1, 2, -1, -1, -1)), ops.OtterHipError),
+                        (lambda: ops.attn_cache_rows(q[:, 0], k[:, 0], k[:1, 0], codes, scales), ValueError), (lambda: ops.kv_cache_write(k, k, codes.cpu(), scales), ops.OtterHipError)):
+        with pytest.raises(error):
+            call()
+    assert ops.attn_cache(q[:0], codes, scales).shape == (0, 1, hq, d) and ops.kv_cache_read(codes, scales, d, 0)[0].shape == (2, 0, h, d)
+    assert bool((codes == 0).all())

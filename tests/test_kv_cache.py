@@ -209,3 +209,19 @@ def test_attention_refuses_what_no_launch_holds():
     # 2^26 rows of one head: one workgroup takes four, a grid has 2^32 threads
     many = _cache(heads=1, episodes=1 << 27)
     _refused(lib.otter_attn_cache(many, _rows(n_rows=1 << 27), 2, _operand(), 1, None, None, _operand(), 1, 0, 16, 0.1, None, 0, None), "grid")
+
+
+def test_the_compiled_way_leaves_what_it_does_not_take():
+    """Anything but whole device tensors of the right kind: None, nothing done, nothing raised."""
+    b = _lib.kv_binding()
+    codes, scales = torch.zeros(2, 1, 1, 4, 16, dtype=torch.uint8), torch.zeros(2, 1, 1, 4, 4, dtype=torch.uint8)
+    x = torch.zeros(1, 1, 1, 32)
+    sparse = torch.zeros(1, 1, 1, 32).to_sparse()
+    for k in (x, x[0], sparse, None, 3, "k", torch.zeros(1, 1, 1, 32, device="meta"), torch.nn.Parameter(x)):
+        for c, s in ((codes, scales), (scales, codes), (None, scales), (codes, sparse), (sparse, sparse), (codes.to("meta"), scales.to("meta"))):
+            assert b.write(k, k, c, s, None, None, None) is None
+            assert b.attend(k, None, None, c, s, None, None, None, True, 0, None, None) is None
+            assert b.attend(k, k, k, c, s, None, None, None, True, 0, None, None) is None
+            assert b.read(c, s, 32, 1, None, None, None, None, 2) is None
+    assert b.write() is None and b.read(codes) is None and b.attend(x, x) is None
+    assert b.read(codes, scales, "32", 1, None, None, None, None, 2) is None and b.read(codes, scales, 1 << 70, 1, None, None, None, None, 2) is None
