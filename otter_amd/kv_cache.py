@@ -16,7 +16,7 @@ quarter of 2^e (2^-10 of 2^e), e the block's exponent.  The arithmetic on the st
 | ``kv_cache_write`` | keys and values -> blocks of codes and scales |
 | ``kv_cache_read`` | blocks -> numbers |
 | ``attn_cache`` | ``softmax(q k^T / sqrt(d)) v`` over the cached positions, one or many new positions a row |
-| ``attn_cache_rows`` | one new position a row: write and attend in one launch |
+| ``attn_cache_rows`` | one new position a row: write and attend in one call |
 """
 from __future__ import annotations
 
