@@ -61,9 +61,13 @@ template <> struct AttnTerms<float> { static constexpr int q = 3, p = 3; };
 
 // Operand types and terms of the two products.  HALF: the values (and, for fp16 activations, the keys: the query is then one exact
 // term) as fp16.  A block's numbers are exact in fp16 if its exponent e leaves them between 2^-24 and 65504: -23 <= e <= 13 for
-// e2m1, -15 <= e <= 7 for e4m3 (magnitudes between about 1e-6 and 5e4); a block at the lowest exponent, -100, is zeros or below
-// 8e-30 and counts as zeros.  A workgroup that meets any other block starts over in bf16 terms.  Weights are scaled by 2^11 (below
-// 2^15 with the reference's growth of 2^4): the smallest fp16 number is then 2^-35 of the largest weight.
+// e2m1 (blocks whose largest number is between 1e-6 and 5e4).  e4m3 has a range of its own, so its numbers are taken 2^kUp times as large:
+// -20 <= e <= 2, largest numbers between 4e-4 and 1.8e3, where -15 <= e would send any key whose values are below 7e-3 the long
+// way (8 windows of 2047 steps, 12 heads of 64 with such keys: fp16 281 us, bf16 215; now 136 and 108).
+// A block at the lowest exponent, -100, is zeros or below 8e-30 and counts as zeros.  A workgroup that meets any other block starts over
+// in bf16 terms.  Weights are scaled by 2^11 (below 2^15 with the reference's growth of 2^4): the smallest fp16 number is then 2^-35
+// of the largest weight.
+template <int BITS> constexpr int kUp = BITS == 8 ? 5 : 0;
 template <typename T, bool HALF> struct Products { typedef __bf16 key, value; static constexpr int q = AttnTerms<T>::q, p = AttnTerms<T>::p; static constexpr float growth = 8.f, lift = 0.f; };
 template <> struct Products<__bf16, true> { typedef __bf16 key; typedef _Float16 value; static constexpr int q = 1, p = 1; static constexpr float growth = 4.f, lift = 11.f; };
 template <> struct Products<_Float16, true> { typedef _Float16 key, value; static constexpr int q = 1, p = 2; static constexpr float growth = 4.f, lift = 11.f; };
@@ -774,6 +778,8 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
     typedef WideTile<NB, BITS> W;
     typedef typename Products<T, HALF>::key K;
     typedef typename Products<T, HALF>::value V;
+    constexpr unsigned key_up = KvElem<K>::code == DT_F16 ? (unsigned)kUp<BITS> << 23 : 0u, value_up = HALF ? (unsigned)kUp<BITS> << 23 : 0u;
+    auto up = [](float scale, unsigned by) { return __uint_as_float(__float_as_uint(scale) + by); };
     const int li = lane & 15, g = lane >> 4;
     auto meet = [&](unsigned word, bool clean) {
 #pragma unroll
@@ -783,15 +789,16 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
             most = max(most, clean && y >= 228u << 24 ? 0u : y);
         }
     };
-    if constexpr (KvElem<K>::code == DT_F16) meet(r.ks, true);     // (not a number: one in either type)
-    if constexpr (HALF) {                                          // (an edge's rows that are not finite are taken out)
-        if (edge) meet(16 * w + li < before ? 0u : r.own, true);
+    if constexpr (HALF) {
+        const bool unseen = edge && 16 * w + li < before;          // (what nobody sees decides nothing; an edge's rows that are not finite are taken out)
+        if constexpr (KvElem<K>::code == DT_F16) meet(unseen ? 0u : r.ks, true);       // (a key that is not a number is one in either type)
+        if (edge) meet(unseen ? 0u : r.own, true);
         else meet(r.own, false);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j)
         *(typename Half16<K>::v8*)(buf + (w * NB + j) * 1024 + lane * 16) =
-            decode8<BITS, K>(&r.k[j * BITS / 4], scale_of(r.ks, NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2));
+            decode8<BITS, K>(&r.k[j * BITS / 4], up(scale_of(r.ks, NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2), key_up));
     if (NB == 1 && (w & 1)) return;
     const int block = NB == 1 ? 0 : NB == 2 ? li >> 3 : NB == 3 ? min(li, 11) >> 2 : li >> 2;
     if (edge) {
@@ -817,7 +824,7 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
     }
     float sc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sc[i] = scale_of(r.vs[i], block);
+    for (int i = 0; i < 8; ++i) sc[i] = up(scale_of(r.vs[i], block), value_up);
     unsigned char* to = buf + (4 * NB + (w >> 1) * W::DV + (w & 1) * 2 * W::PW) * 1024 + lane * 16;
 #pragma unroll
     for (int j = 0; j < W::PW; ++j) {
@@ -848,6 +855,7 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
     load_queries<NB, T, QT, HALF>(a, i, h, col, g, qf);
     st.reset();
     float mark[QT] = {};
+    constexpr float key_down = KvElem<typename P::key>::code == DT_F16 ? 1.f / (1 << kUp<BITS>) : 1.f;      // scores come out 2^kUp times as large
     f32x4 lsum[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) lsum[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -888,7 +896,7 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
                         for (int t = 0; t < QT; ++t) s[t][hh] = HK::mfma32(kf, qf[t][n][j], s[t][hh]);
                     }
             const bool masked = k0 + 63 > own.hi_all || k0 + 64 > stop || k0 < own.lo_all;
-            tile_weights<NB, BITS, T, QT, 2, HALF>(s, st, pf, lsum, k0, masked, lo, hi, a.c, lane);
+            tile_weights<NB, BITS, T, QT, 2, HALF>(s, st, pf, lsum, k0, masked, lo, hi, a.c * key_down, lane);
         }
         if (more) {                                                // the next tile into the other buffer, the one behind it on its way
             wide_convert<NB, BITS, T, HALF>(raw, lds + (at ^ 1) * W::bytes, edge(k0 + 64), kr.beg - k0 - 64, least, most, lane, w);
@@ -928,15 +936,17 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
         __syncthreads();
     }
     if constexpr (HALF) {
-        constexpr int lo_byte = BITS == 4 ? 127 - 23 : 127 - 15, hi_byte = BITS == 4 ? 127 + 13 : 127 + 7;
+        constexpr int lo_byte = (BITS == 4 ? 127 - 23 : 127 - 15) - kUp<BITS>, hi_byte = (BITS == 4 ? 127 + 13 : 127 + 7) - kUp<BITS>;
         if (__syncthreads_or(least < (lo_byte - 28u) << 24 || most >= (hi_byte + 1u) << 24)) return true;
     }
-    const float down = HALF ? __builtin_amdgcn_exp2f(-P::lift) : 1.f;       // (exact: splits of one column may be of either kind)
+    // (exact: splits of one column may be of either kind)
+    constexpr float down = HALF ? 1.f / (1 << (int)P::lift) : 1.f, value_down = HALF ? down / (1 << kUp<BITS>) : 1.f;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
+        st.m[t] *= key_down;
         st.l[t] = (kSumByProduct<T, HALF> ? lsum[t][0] : rows_sum(st.l[t])) * down;      // (the product's sum is over all keys already)
 #pragma unroll
-        for (int j = 0; j < DV; ++j) st.acc[t][j] = st.acc[t][j] * down + mark[t];
+        for (int j = 0; j < DV; ++j) st.acc[t][j] = st.acc[t][j] * value_down + mark[t];
     }
     return false;
 }
