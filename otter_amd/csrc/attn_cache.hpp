@@ -177,6 +177,12 @@ __device__ __forceinline__ float scale_of(unsigned word, int block) {
     const unsigned rot = (unsigned)(9 + 8 * block) & 31u;         // rotate right by 9 + 8 b: byte b lands on bits 23 .. 30
     return __uint_as_float(__builtin_amdgcn_alignbit(word, word, rot));
 }
+// the same times 2^UP; the addition stops at the byte 255, which says that the block is no number
+template <int UP> __device__ __forceinline__ float scale_up(unsigned word, int block) {
+    if constexpr (UP == 0) return scale_of(word, block);
+    const unsigned rot = (unsigned)(8 + 8 * block) & 31u;         // byte b on bits 24 .. 31
+    return __uint_as_float(__builtin_elementwise_add_sat(__builtin_amdgcn_alignbit(word, word, rot), (unsigned)UP << 24) >> 1);
+}
 
 // pair number j of a lane's words as two numbers of type V
 template <int BITS, typename V = __bf16> __device__ __forceinline__ unsigned decode_pair(const unsigned* w, int j, float sc) {
@@ -778,27 +784,27 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
     typedef WideTile<NB, BITS> W;
     typedef typename Products<T, HALF>::key K;
     typedef typename Products<T, HALF>::value V;
-    constexpr unsigned key_up = KvElem<K>::code == DT_F16 ? (unsigned)kUp<BITS> << 23 : 0u, value_up = HALF ? (unsigned)kUp<BITS> << 23 : 0u;
-    auto up = [](float scale, unsigned by) { return __uint_as_float(__float_as_uint(scale) + by); };
+    constexpr int key_up = KvElem<K>::code == DT_F16 ? kUp<BITS> : 0, value_up = HALF ? kUp<BITS> : 0;
     const int li = lane & 15, g = lane >> 4;
-    auto meet = [&](unsigned word, bool clean) {
+    auto meet = [&](unsigned word, unsigned passes) {              // blocks whose byte is `passes` or more have no say
 #pragma unroll
         for (int b = 0; b < NB; ++b) {                             // (what lies below the byte decides nothing)
             const unsigned y = word << (24 - 8 * b);
-            least = min(least, clean && y >= 228u << 24 ? ~0u : y - (28u << 24));
-            most = max(most, clean && y >= 228u << 24 ? 0u : y);
+            const bool pass = passes < 256u && y >= passes << 24;
+            least = min(least, pass ? ~0u : y - (28u << 24));
+            most = max(most, pass ? 0u : y);
         }
     };
     if constexpr (HALF) {
         const bool unseen = edge && 16 * w + li < before;          // (what nobody sees decides nothing; an edge's rows that are not finite are taken out)
-        if constexpr (KvElem<K>::code == DT_F16) meet(unseen ? 0u : r.ks, true);       // (a key that is not a number is one in either type)
-        if (edge) meet(unseen ? 0u : r.own, true);
-        else meet(r.own, false);
+        if constexpr (KvElem<K>::code == DT_F16) meet(unseen ? 0u : r.ks, 255u);       // (a key that is no number is none in either type)
+        if (edge) meet(unseen ? 0u : r.own, 228u);
+        else meet(r.own, 256u);
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j)
         *(typename Half16<K>::v8*)(buf + (w * NB + j) * 1024 + lane * 16) =
-            decode8<BITS, K>(&r.k[j * BITS / 4], up(scale_of(r.ks, NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2), key_up));
+            decode8<BITS, K>(&r.k[j * BITS / 4], scale_up<key_up>(r.ks, NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2));
     if (NB == 1 && (w & 1)) return;
     const int block = NB == 1 ? 0 : NB == 2 ? li >> 3 : NB == 3 ? min(li, 11) >> 2 : li >> 2;
     if (edge) {
@@ -824,7 +830,7 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
     }
     float sc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sc[i] = up(scale_of(r.vs[i], block), value_up);
+    for (int i = 0; i < 8; ++i) sc[i] = scale_up<value_up>(r.vs[i], block);
     unsigned char* to = buf + (4 * NB + (w >> 1) * W::DV + (w & 1) * 2 * W::PW) * 1024 + lane * 16;
 #pragma unroll
     for (int j = 0; j < W::PW; ++j) {
