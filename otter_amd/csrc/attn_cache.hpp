@@ -64,8 +64,8 @@ template <> struct AttnTerms<float> { static constexpr int q = 3, p = 3; };
 // e2m1 (blocks whose largest number is between 1e-6 and 5e4).  e4m3 has a range of its own, so its numbers are taken 2^kUp times as large:
 // -20 <= e <= 2, largest numbers between 4e-4 and 1.8e3, where -15 <= e would send any key whose values are below 7e-3 the long
 // way (8 windows of 2047 steps, 12 heads of 64 with such keys: fp16 281 us, bf16 215; now 136 and 108).
-// A block at the lowest exponent, -100, is zeros or below 8e-30 and counts as zeros.  A workgroup that meets any other block starts over
-// in bf16 terms.  Weights are scaled by 2^11 (below 2^15 with the reference's growth of 2^4): the smallest fp16 number is then 2^-35
+// A workgroup that meets any other block that holds numbers starts over in bf16 terms (a block of zeros has the lowest exponent, -100: where
+// scale bytes below the range were met, the codes decide).  Weights are scaled by 2^11 (below 2^15 with the reference's growth of 2^4): the smallest fp16 number is then 2^-35
 // of the largest weight.
 template <int BITS> constexpr int kUp = BITS == 8 ? 5 : 0;
 template <typename T, bool HALF> struct Products { typedef __bf16 key, value; static constexpr int q = AttnTerms<T>::q, p = AttnTerms<T>::p; static constexpr float growth = 8.f, lift = 0.f; };
@@ -777,8 +777,8 @@ template <int NB, int BITS, bool HALF> __device__ __forceinline__ void wide_load
 
 // `edge`: the tile has keys that some column does not see: blocks that are not finite are taken out and named in the masks; so are
 // the tile's first `before` rows, which no column sees
-// `least`, `most`: over the scale bytes of the tile's keys (a wave looks at its 16), as the top bits of a word, `least` less 28: the
-// lowest exponent's byte 27 and the zeros of rows that do not exist wrap around and pass
+// `least`, `most`: over the scale bytes of the tile's keys (a wave looks at its 16), as the top bits of a word, `least` less 1: the
+// zeros of rows that do not exist wrap around and pass
 template <int NB, int BITS, typename T, bool HALF>
 __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned char* buf, bool edge, int before, unsigned& least, unsigned& most, int lane, int w) {
     typedef WideTile<NB, BITS> W;
@@ -791,7 +791,7 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
         for (int b = 0; b < NB; ++b) {                             // (what lies below the byte decides nothing)
             const unsigned y = word << (24 - 8 * b);
             const bool pass = passes < 256u && y >= passes << 24;
-            least = min(least, pass ? ~0u : y - (28u << 24));
+            least = min(least, pass ? ~0u : y - (1u << 24));
             most = max(most, pass ? 0u : y);
         }
     };
@@ -844,6 +844,30 @@ __device__ __forceinline__ void wide_convert(WideTile<NB, BITS>& r, unsigned cha
         *(u32x4*)(to + 2 * j * 1024) = vf[0];
         *(u32x4*)(to + (2 * j + 1) * 1024) = vf[1];
     }
+}
+
+// whether a block of rows beg .. stop - 1 whose scale byte is below LO holds a number other than zero.  Read again only after a walk that met
+// such bytes: 8 windows of 2047 steps, 12 heads of 64, with zeros in every 50th row take 110 us (bf16, 4 bits) and 141 (fp16, 8 bits), without
+// any 105 and 119; a second walk costs 100 and more.
+template <int NB, int BITS, int LO>
+__device__ __forceinline__ bool low_numbers(const unsigned char* rows, const unsigned char* scales, int start, int stop, int beg, int lane, int w) {
+    constexpr int RB = 4 * NB * BITS, KB = RB / 4;
+    constexpr unsigned magnitude = BITS == 4 ? 0x77777777u : 0x7f7f7f7fu;
+    asm volatile("" : "+v"(lane), "+s"(start), "+s"(stop));        // (nothing of this is worth a register of the walk before it)
+    const int li = lane & 15, g = lane >> 4;
+    bool found = false;
+    for (int k0 = start + 16 * w; k0 < stop; k0 += 64) {           // a wave takes 16 rows, a lane a quarter of one
+        unsigned c[RawTile<NB, BITS>::KW];
+        buffer_words<KB>(rows_of(rows, k0, RB, stop - k0), li * RB + g * KB, c);
+        const unsigned word = __builtin_amdgcn_raw_buffer_load_b32(rows_of(scales, k0, 4, stop - k0), li * 4, 0, 0);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {                             // (units of 8 numbers, as in tile_scores)
+            const int block = NB == 1 ? 0 : NB == 2 ? g >> 1 : NB == 4 ? g : (3 * g + j) >> 2;
+            const unsigned some = (c[j * BITS / 4] | c[j * BITS / 4 + BITS / 4 - 1]) & magnitude;
+            found |= some != 0u && (word >> (8 * block) & 255u) < LO && k0 + li >= beg;
+        }
+    }
+    return found;
 }
 
 // a workgroup's walk over its keys; true: a block does not fit the fp16 operands, the state is void (the same for all threads)
@@ -943,7 +967,12 @@ __device__ __forceinline__ bool wide_walk(const AttnCacheArgs& a, const TileSour
     }
     if constexpr (HALF) {
         constexpr int lo_byte = (BITS == 4 ? 127 - 23 : 127 - 15) - kUp<BITS>, hi_byte = (BITS == 4 ? 127 + 13 : 127 + 7) - kUp<BITS>;
-        if (__syncthreads_or(least < (lo_byte - 28u) << 24 || most >= (hi_byte + 1u) << 24)) return true;
+        if (__syncthreads_or(most >= (hi_byte + 1u) << 24)) return true;
+        if (__builtin_expect(__syncthreads_or(least < (lo_byte - 1u) << 24), 0)) {       // (rare: zeros, or numbers that the operands have lost)
+            bool lost = low_numbers<NB, BITS, lo_byte>(src.v, src.vs, start, stop, kr.beg, lane, w);
+            if constexpr (KvElem<typename P::key>::code == DT_F16) lost |= low_numbers<NB, BITS, lo_byte>(src.k, src.ks, start, stop, kr.beg, lane, w);
+            if (__syncthreads_or(lost)) return true;
+        }
     }
     // (exact: splits of one column may be of either kind)
     constexpr float down = HALF ? 1.f / (1 << (int)P::lift) : 1.f, value_down = HALF ? down / (1 << kUp<BITS>) : 1.f;
