@@ -584,7 +584,7 @@ __global__ __launch_bounds__(256, narrow_groups(KvElem<T>::code, NB, QT)) void a
     constexpr int D = 32 * NB, RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, NQ = AttnTerms<T>::q;
     constexpr int MROW = D + 4;                                    // padded row of the merge buffer
     __shared__ __attribute__((aligned(16))) unsigned char fresh_rows[4][2 * RB + 16];
-    __shared__ float merge[4 * 16 * MROW];
+    __shared__ __attribute__((aligned(16))) float merge[4 * 16 * MROW];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, g = lane >> 4;
     const int U = a.g.n * a.g.H;
