@@ -182,6 +182,9 @@ def kv_binding():
             from . import _kv_binding as b
         except ImportError as e:
             raise OtterHipError(f"{os.path.join(_HERE, '_kv_binding.so')} cannot be loaded ({e}): build it with `make -C otter_amd/csrc`") from e
+        built = getattr(b, "ABI_VERSION", None)
+        if built != ABI_VERSION:
+            raise OtterHipError(f"{os.path.join(_HERE, '_kv_binding.so')} has ABI version {built}, expected {ABI_VERSION}: build it with `make -C otter_amd/csrc`")
         names = ("otter_kv_cache_write", "otter_kv_cache_read", "otter_attn_cache", "otter_attn_cache_workspace_floats")
         b.bind(*(ctypes.cast(getattr(lib, n), c_void_p).value for n in names), torch._C._cuda_getCurrentRawStream)
         _binding = b

@@ -224,4 +224,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_kv_binding", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__kv_binding(void) { return PyModule_Create(&module); }
+// (the structs' layouts and the entry points' signatures are compiled in: _lib.py compares their version before it binds)
+PyMODINIT_FUNC PyInit__kv_binding(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddIntConstant(m, "ABI_VERSION", OTTER_HIP_ABI_VERSION) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}
