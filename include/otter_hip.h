@@ -366,6 +366,9 @@ int otter_kv_cache_read(const otter_kv_cache* cache, const otter_kv_rows* rows, 
  * only those below max_len (what the caller knows about its lengths; capacity if nothing) and capacity.  A query that sees
  * nothing, and every t >= count[i], gives zeros.  q, out: q_heads heads, a multiple of the cache's; query head j reads key head
  * j / (q_heads / heads).  fp16: cut at +-65504.
+ * Scores, sums and accumulators are fp32 (scale * q.k has to stay within it).  A weight of the sum over the values is rounded by at
+ * most 2^-24 of itself for fp32 activations and 2^-16 for 16-bit ones, but 2^-11 for bf16 ones with more than 32 columns (steps * q_heads /
+ * heads) and several steps, an eighth of the output's own half step; there, weights below 2^-25 of a row's largest are rounded by at most 2^-36 of that.
  * k_new / v_new (both or none; steps == 1, count NULL): the step's own key and value, quantised, stored at pos[e] and attended to by the
  * same launch -- as otter_kv_cache_write followed by this call.
  * workspace: otter_attn_cache_workspace_floats(...) floats (max_len there: no more than the capacity), 8-byte aligned, private to

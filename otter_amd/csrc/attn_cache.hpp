@@ -5,10 +5,14 @@
 //
 // Operands.  A stored number has at most 4 significant bits, so k_j and v_j are exact in bf16 and the products run on
 // v_mfma_f32_16x16x32_bf16 with fp32 accumulation.  q and p are written as sums of bf16 terms: q exactly (1 term for bf16, 2 for
-// fp16, 3 for fp32), p in 2 terms (2^-17 relative, far below the output's own rounding) for 16-bit and 3 (2^-24) for fp32 outputs.
+// fp16, 3 for fp32), p in 2 terms (2^-16 relative, far below the output's own rounding) for 16-bit and 3 (2^-24) for fp32 outputs.
 //
 // For 16-bit activations and many columns the second product runs on fp16 operands instead, as long as the values allow it (see
-// `Products`): fp16 weights carry 2^-12, so that bf16 outputs need one term where bf16 weights need two.
+// `Products`): one fp16 term is off by at most 2^-11 of a weight (an eighth of a bf16 output's own half step, 2^-8; numerator and
+// denominator take the same rounded weight), so bf16 outputs need one term where bf16 weights need two; fp16 outputs take two, 2^-22.
+// With one term 8 % of bf16 outputs are the neighbour of the rounded result, with two 0.04 %; the error against 64 bits is 1.6e-3 of the norm
+// with either, that of the output's rounding.  The second term costs 124 against 107 us (8 windows of 2047) and 472 against 397 (500-step
+// chunk).  A caller that wants every bit passes fp32 activations (2^-24 throughout).
 //
 // Tile.  A wave owns 16 * QT columns (query positions x heads of one key head's group) and walks over tiles of 32 keys, all
 // state in registers.  S^T = K Q^T puts 8 scores of one column in a lane, keys 4g+i and 16+4g+i (g = lane / 16), which is the
@@ -579,6 +583,8 @@ __device__ __forceinline__ int append_row(const AttnCacheArgs& a, const KvRow& r
 // Memory-bound where it matters, one position over long histories: 48 rows x 32 / 8 heads of 128 over 7001 to 16383 positions in 4 bits
 // read 610 MB in 126 us (4.8 TB/s, the rate of a large copy), 160 x 16 / 4 heads of 64 over the last 1000 in 8 bits 85 MB in 20 us.
 // Short windows (64 x 8 heads x 32 steps of 96, fp32: 9 us) are one tile a wave: the latency of its dependent loads.
+// Registers spilled under the launch bounds: fp16 heads of 128, 2 (4 bits) and 13 (8 bits) with 16 columns, 14 (8 bits) with 32; fp32 heads of 96, 2
+// and 10; none elsewhere.
 template <int NB, int BITS, typename T, int QT>
 __global__ __launch_bounds__(256, narrow_groups(KvElem<T>::code, NB, QT)) void attn_cache_kernel(AttnCacheArgs a) {
     constexpr int D = 32 * NB, RB = 4 * NB * BITS, DV = RawTile<NB, BITS>::DV, NQ = AttnTerms<T>::q;
@@ -740,9 +746,13 @@ __global__ __launch_bounds__(256, narrow_groups(KvElem<T>::code, NB, QT)) void a
 // which the matrix operands are read (16 bytes a lane, no conflicts), while the previous tile is being multiplied: two buffers,
 // one barrier a tile.
 // A tile of 64 keys x 32 columns x 64 numbers is 36 products (576 cycles) and 190 vector instructions a wave in bf16, 32 of them
-// exponentials, and the two hardly overlap.  8 windows of 2047 steps, 12 heads of 64, 4 bits: bf16 100 us (820 TFLOP/s of the whole
-// tiles, 512 counting only visible keys), fp16 131, fp32 174; 8 x 500 steps after 2500 to 7600 positions, 32 / 8 heads of 128, bf16
-// 400 us (810 TFLOP/s).  With a kernel of the narrow form the two took 158 and 767 us.
+// exponentials.  8 windows of 2047 steps, 12 heads of 64, 4 bits: bf16 100 to 106 us by the machine (512 TFLOP/s at 100, counting only visible
+// keys), fp16 131, fp32 174; 8 x 500 steps after 2500 to 7600 positions, 32 / 8 heads of 128, bf16 395 us.  With a kernel of the narrow
+// form the two took 158 and 767 us.  Bound by vector issue and waiting: of a SIMD's cycles 21 % are products and 41 % the issue of vector
+// instructions (the exponentials take longer than counted there) in the first, 35 and 32 % in the second, and the waves wait a third.
+// Products do not exclude vector instructions (from another wave about half of an exponential, maximum and fma mix hides behind them); more waves
+// a SIMD do not fit the accumulators, and the fp16 kernels of two column groups for heads of 64 already spill (33 registers in 4 bits, 43 in 8:
+// the bf16 walk that they contain needs two query terms).
 template <int NB, int BITS> struct WideTile {
     static constexpr int DV = RawTile<NB, BITS>::DV, KW = RawTile<NB, BITS>::KW;
     static constexpr int PW = DV / 4 > 0 ? DV / 4 : 1;             // pairs of numbers of a value row that one wave converts

@@ -10,7 +10,9 @@ namespace {
 // along the heads: a cache row is contiguous with the row of the next step, so a wave's codes form one run, and its numbers runs
 // of head_dim elements.  Memory-bound: head_dim * (element size + BITS / 8) + 4 bytes a row, no reuse; a lane takes up to four
 // pieces whose loads are requested together, and the four scale bytes of a row leave in one store.  16 x 4093 steps x 8 heads of
-// 128 between bf16 and 4 bits: write 72 us (4.7 TB/s), read 66 us (5.1); 24 x 6001 x 8 heads of 64, fp16: 78 and 75 us (4.8, 5.0).
+// 128 between bf16 and 4 bits, 339 MB: write 63 us on the same numbers again, 73 on others each time (4.6 TB/s), 90 behind a read-back, whose 268 MB
+// of results fill the last-level cache (256 MB) and have to leave it; read 55 us (6.1 TB/s: the codes, 71 MB, stay in that cache).  24 x 6001 x 8 heads of 64,
+// fp16, 373 MB: 78 and 71 us.  Copies reach 7.0 TB/s of 2 x 128 MB (inside the cache), 5.4 of 2 x 256 MB and 4.8 of 2 x 2 GB.
 template <int NB> struct RowLanes { static constexpr int P = NB == 1 ? 4 : NB == 2 ? 8 : 16, live = 4 * NB; };
 
 template <int NB, int BITS, typename T, int M, int MH>
@@ -176,8 +178,8 @@ void launch_m(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand
 
 // One piece a lane while that leaves the chip short of workgroups, four otherwise.  A wave that writes takes the same four rows of
 // four heads where the heads allow: it reads runs of four heads (one projection's output holds q | k | v of a step, so a head alone
-// is 256 bytes of 6 KB): 16 histories of 4093 steps x 8 heads of 128, bf16 -> 4 bits 72 us against 86 with sixteen rows of one head.  Reading
-// is as fast or faster along one head (56 us against 60).
+// is 256 bytes of 6 KB): 16 histories of 4093 steps x 8 heads of 128, bf16 -> 4 bits 72 us against 86 with sixteen rows of one head (other numbers
+// each time).  Reading is as fast or faster along one head (56 us against 60).
 template <bool WRITE, int NB, int BITS, typename T>
 void launch(const KvGeom& g, const otter_kv_operand* k, const otter_kv_operand* v, int vec, hipStream_t s) {
     if ((long)g.H * g.T * RowLanes<NB>::P / 1024 * 2 * g.n >= 2048) {

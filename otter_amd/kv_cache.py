@@ -9,7 +9,9 @@ in 4 bits (e2m1 codes), 1.6 kB in 8 (e4m3), and histories of any length.  Number
 
 Accuracy is the format's, half a step of the code: a number that is stored in 4 bits is within a fifth of itself if it is at least a
 sixth of its block's largest, in 8 bits within 2^-4 of itself if it is at least 2^-14 of the largest; smaller ones are within a
-quarter of 2^e (2^-10 of 2^e), e the block's exponent.  The arithmetic on the stored numbers is that of the activations' type (fp32 activations: fp32).
+quarter of 2^e (2^-10 of 2^e), e the block's exponent.  The arithmetic on the stored numbers is fp32 for fp32 activations; for 16-bit ones scores
+and sums are fp32 and a weight is held to 2^-16, or 2^-11 for bf16 activations with several steps and more than 32 columns (steps x
+query heads of a key head), below the output's own rounding (2^-8).
 
 | operator | arithmetic |
 |---|---|
