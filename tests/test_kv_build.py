@@ -34,3 +34,13 @@ def test_a_binding_of_another_version_is_refused(monkeypatch, version):
     assert not bound and _lib._binding is None
     monkeypatch.undo()
     assert _lib.kv_binding().ABI_VERSION == _lib.ABI_VERSION
+
+
+def test_build_compiles_what_is_already_there(monkeypatch):
+    """build() is the check that the sources compile: objects that exist do not count as built."""
+    import __graft_entry__ as entry
+    ran = []
+    monkeypatch.setattr(entry.subprocess, "run", lambda cmd, **kw: ran.append((cmd, kw)))
+    entry.build()
+    (cmd, kw), = ran
+    assert cmd[0] == "make" and "-B" in cmd and kw.get("check") is True
